@@ -154,7 +154,7 @@ def _quantise(x):
     amax = torch.where(finite, x.abs(), torch.zeros_like(x)).amax(-1)
     # amax = m * 2^e with m in [0.5, 1); 448 = 0.875 * 2^9
     m, e = torch.frexp(amax)
-    e = (e - 9 + (m > 0.875).to(e.dtype)).clamp(-120, 120)
+    e = (e - 9 + (m > 0.875).to(e.dtype)).clamp(-120, 119)
     e = torch.where(amax == 0, torch.zeros_like(e), e)
     y = (x * _pow2(-e)[..., None]).clamp(-E4M3_MAX, E4M3_MAX)
     return y.to(torch.float8_e4m3fn), e.to(torch.int8)
@@ -398,7 +398,7 @@ def _exact_round(x):
     amax = x.abs().amax(-1, keepdim=True)
     e = torch.ceil(torch.log2(amax.clamp(min=1e-300) / 448.0))
     e = torch.where(amax > 448.0 * _wide_pow2(e), e + 1, e)
-    e = torch.where(amax <= 448.0 * _wide_pow2(e - 1), e - 1, e).clamp(-120, 120)
+    e = torch.where(amax <= 448.0 * _wide_pow2(e - 1), e - 1, e).clamp(-120, 119)
     y = x / _wide_pow2(e)
     # 3 mantissa bits, the least normal exponent -6: spacing 2^(floor(log2 |y|) - 3)
     _, k = torch.frexp(y)
