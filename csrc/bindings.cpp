@@ -128,6 +128,24 @@ void ep_return(torch::Tensor rows, torch::Tensor cnt, torch::Tensor peers, int64
                int64_t cap);
 void ep_combine(torch::Tensor ret, c10::optional<torch::Tensor> w, torch::Tensor topi, torch::Tensor pos,
                 torch::Tensor starts, torch::Tensor out, int64_t cap);
+// cached decoding
+void kv_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Tensor v_cache,
+                    c10::optional<torch::Tensor> k_exp, c10::optional<torch::Tensor> v_exp, torch::Tensor starts,
+                    c10::optional<torch::Tensor> counts);
+void kv_cache_read(torch::Tensor k_cache, torch::Tensor v_cache, c10::optional<torch::Tensor> k_exp,
+                   c10::optional<torch::Tensor> v_exp, torch::Tensor starts, torch::Tensor k_out,
+                   torch::Tensor v_out);
+void decode_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::optional<torch::Tensor> k_exp,
+                      c10::optional<torch::Tensor> v_exp, c10::optional<torch::Tensor> pk,
+                      c10::optional<torch::Tensor> pv, c10::optional<torch::Tensor> pk_exp,
+                      c10::optional<torch::Tensor> pv_exp, torch::Tensor lengths, c10::optional<torch::Tensor> counts,
+                      int64_t window, double scale, torch::Tensor out);
+void kda_recurrent(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor g, torch::Tensor beta, double scale,
+                   c10::optional<torch::Tensor> s0, c10::optional<torch::Tensor> counts, torch::Tensor o,
+                   torch::Tensor s1);
+void verify_draft(torch::Tensor target, c10::optional<torch::Tensor> draft, torch::Tensor tokens, torch::Tensor uniform,
+                  torch::Tensor noise, c10::optional<torch::Tensor> lens, c10::optional<torch::Tensor> temperature,
+                  double temp, torch::Tensor out, torch::Tensor accepted, torch::Tensor logp);
 }  // namespace hb
 
 static int64_t read_status() {
@@ -222,4 +240,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ep_zero_pads", &hb::ep_zero_pads);
   m.def("ep_return", &hb::ep_return);
   m.def("ep_combine", &hb::ep_combine);
+  m.def("kv_cache_write", &hb::kv_cache_write);
+  m.def("kv_cache_read", &hb::kv_cache_read);
+  m.def("decode_attention", &hb::decode_attention);
+  m.def("kda_recurrent", &hb::kda_recurrent);
+  m.def("verify_draft", &hb::verify_draft);
 }

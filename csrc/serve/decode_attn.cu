@@ -1,0 +1,818 @@
+// Attention of a few new tokens per sequence over cached keys and values, with a
+// prefix that the whole batch shares.
+//
+// Query (b, i, h), i < counts[b], stands at pos = P + lengths[b] - counts[b] + i
+// and sees prefix keys j (at j) and the sequence's own keys j (at P + j) with
+// kpos <= pos and, with a window W > 0, pos - kpos < W.
+//   o = sum_j 2^{s_j - m} v_j / sum_j 2^{s_j - m},   s_j = scale log2(e) q.k_j
+// One pass over the keys with the running maximum m and sum l of every row.  The
+// keys are split into pieces; each piece leaves (O, m, l) of its rows in fp32
+// and decode_combine_kernel joins them:  o = sum_p 2^{m_p - M} O_p / sum_p 2^{m_p - M} l_p.
+//
+// Own keys: all G = Nq / Nkv heads and all S tokens of a sequence share its keys,
+// so a CTA holds S * G rows (16 MT at a time) of one KV head.  The 32-key tiles
+// of all sequences are laid end to end and cut into equal ranges, one per CTA, so
+// ragged lengths balance; piece (CTA c, sequence b) has slot c + b, since going
+// along the tiles each new piece starts a new CTA or a new sequence.
+// Prefix keys: the rows of all sequences (B * S * G of a KV head) are queries of
+// one long sequence: row tiles x key splits.
+//
+// A CTA is 4 warps that share the rows and take every fourth 32-key tile, each
+// with its own cp.async ring, m, l and O (no barrier between tiles); they merge
+// through shared memory at the end of a piece.  Products on mma.sync: at S * G
+// rows the tensor work is small against the bytes of the keys.
+//
+// A quantised cache holds e4m3 codes and a power-of-two exponent per row.  The
+// codes convert to f16 exactly.  q (bf16) enters as f16 scaled per row by a power
+// of two to [2^14, 2^15): exact but for values 2^-25 below the row's largest.
+// Key exponents multiply the scores; value exponents e_j enter the weights, and
+// O has a running maximum of its own, mo = max (s_j + e_j): the f16 weights
+// 2^{s_j + e_j - mo} stay <= 1 whatever the exponents, and O 2^{mo - m} is in the
+// unit of l at the end.
+#include <torch/extension.h>
+
+#include "../common/host.h"
+#include "mma.cuh"
+
+namespace hb {
+namespace {
+
+constexpr int WARPS = 4;
+constexpr int KB = 32;   // keys per warp tile
+constexpr float LOG2E_D = 1.4426950408889634f;
+
+struct KvView {
+  const uint8_t *k, *v;
+  const int8_t *ke, *ve;
+  long long kb, ks, kn, vb, vs, vn;          // bytes
+  long long keb, kes, ken, veb, ves, ven;    // elements
+};
+struct AttnParams {
+  const __nv_bfloat16* q;
+  long long qb, qs, qh;
+  KvView own, pre;
+  const int *lengths, *counts;
+  int B, S, Nq, N, G, C, P, W;
+  int pre_lo;                 // first prefix key that any query can see
+  float sl2;
+  int n_pre, n_split, pre_rt; // prefix CTAs; key splits; row tiles
+  int n_suf, own_rt;          // own-key CTAs per (KV head, row tile); row tiles of a sequence
+  float *own_o, *own_ml, *pre_o, *pre_ml;
+  int* tile_start;            // [B + 1]
+  __nv_bfloat16* out;         // [B, S, Nq, H] contiguous
+  int* status;
+};
+
+HB_DEVICE float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^e for integers, 0 below the normal range.
+HB_DEVICE float pow2c(int e) { return e < -126 ? 0.f : __int_as_float((min(e, 127) + 127) << 23); }
+
+HB_DEVICE int len_of(const AttnParams& p, int b, bool report) {
+  const int x = p.lengths[b], y = min(max(x, 0), p.C);
+  if (report && x != y) set_error(p.status, kErrBounds);
+  return y;
+}
+HB_DEVICE int count_of(const AttnParams& p, int b, int len, bool report) {
+  if (!p.counts) return min(p.S, len);
+  const int x = p.counts[b], y = min(max(x, 0), min(p.S, len));
+  if (report && x != y) set_error(p.status, kErrBounds);
+  return y;
+}
+// First own key that any query of the sequence sees.
+HB_DEVICE int own_lo(const AttnParams& p, int len, int cnt) { return p.W > 0 ? max(0, len - cnt - p.W + 1) : 0; }
+HB_DEVICE int tiles_of(const AttnParams& p, int len, int cnt) {
+  return cnt > 0 ? (len - own_lo(p, len, cnt) + KB - 1) / KB : 0;
+}
+
+template <int H, bool Q8, int MT>
+struct Cfg {
+  static constexpr int RB = Q8 ? H : 2 * H;             // bytes of a cached row
+  static constexpr int CPR = RB / 16;                   // 16-byte chunks of it
+  static constexpr int TILE = KB * RB;                  // K or V tile
+  static constexpr int ST = RB >= 256 ? 3 : 4;          // ring stages
+  static constexpr int RING = ST * 2 * TILE;            // per warp
+  static constexpr int QF = MT * (H / 16) * 32 * 16;    // query fragments
+  static constexpr int MERGE = WARPS * MT * 16 * (H + 4) * 4;
+  static constexpr int BODY = WARPS * RING > MERGE ? WARPS * RING : MERGE;
+  static constexpr int SMEM = QF + MT * 16 * 4 + BODY;
+};
+
+// Byte offset of (key row r, 16-byte chunk c) in a tile: swizzled so that the
+// fragment loads below touch every bank once.
+template <int H, bool Q8>
+HB_DEVICE int tile_off(int r, int c) {
+  constexpr int RB = Q8 ? H : 2 * H;
+  if constexpr (!Q8) return r * RB + ((H == 32 ? c ^ ((r >> 1) & 3) : c ^ (r & 7)) << 4);
+  else if constexpr (H == 64) return (r ^ ((r >> 1) & 1)) * RB + (c << 4);
+  else if constexpr (H == 128) return r * RB + ((c ^ ((r & 1) << 2)) << 4);
+  else return r * RB + (c << 4);
+}
+
+template <int H, bool Q8, int MT>
+__global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParams p) {
+  using F = Cfg<H, Q8, MT>;
+  constexpr int KS = H / 16;        // k16 steps of q.k
+  constexpr int NT = KB / 8;        // score tiles of 8 keys
+  constexpr int JN = H / 8;         // output tiles of 8 columns
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint4* sQ = reinterpret_cast<uint4*>(smem);
+  float* sScale = reinterpret_cast<float*>(smem + F::QF);   // per row: q's exponent and the softmax scale
+  uint8_t* body = smem + F::QF + MT * 16 * 4;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int SG = p.S * p.G;
+  const bool is_pre = (int)blockIdx.x < p.n_pre;
+
+  int n, rt, b = 0, c = 0, tile0, tile1, first_tile = 0;   // tile range of this CTA; first tile of sequence b
+  int len = 0, cnt = 0;
+  if (is_pre) {
+    int x = blockIdx.x;
+    rt = x % p.pre_rt, x /= p.pre_rt;
+    n = x % p.N;
+    c = x / p.N;
+    const int total = (p.P - p.pre_lo + KB - 1) / KB, per = (total + p.n_split - 1) / p.n_split;
+    tile0 = min(c * per, total), tile1 = min(tile0 + per, total);
+  } else {
+    int x = blockIdx.x - p.n_pre;
+    rt = x % p.own_rt, x /= p.own_rt;
+    n = x % p.N;
+    c = x / p.N;
+    // tiles of all sequences: total, and the sequence that holds this CTA's first tile
+    const bool report = blockIdx.x == p.n_pre;
+    __shared__ int wsum[WARPS];
+    int total = 0;
+    for (int b0 = 0; b0 < p.B; b0 += WARPS * 32) {
+      int v = 0;
+      if (b0 + tid < p.B) {
+        const int l = len_of(p, b0 + tid, report);
+        v = tiles_of(p, l, count_of(p, b0 + tid, l, report));
+      }
+      int s = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
+      }
+      __syncthreads();
+      if (lane == 31) wsum[warp] = s;
+      __syncthreads();
+      int base = total;
+      for (int w = 0; w < warp; ++w) base += wsum[w];
+      if (report && b0 + tid < p.B) p.tile_start[b0 + tid] = base + s - v;
+      total += wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    }
+    if (report && tid == 0) p.tile_start[p.B] = total;
+    const int per = max(WARPS, (total + p.n_suf - 1) / p.n_suf);
+    tile0 = min(c * per, total), tile1 = min(tile0 + per, total);
+    if (tile0 >= tile1) return;
+    // second walk: every warp finds the sequence by itself
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      int v = 0;
+      if (b0 + lane < p.B) {
+        const int l = len_of(p, b0 + lane, false);
+        v = tiles_of(p, l, count_of(p, b0 + lane, l, false));
+      }
+      int s = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, first_tile + s > tile0);
+      if (past) {
+        const int k = __ffs(past) - 1;
+        b = b0 + k;
+        first_tile += __shfl_sync(0xffffffffu, s - v, k);
+        break;
+      }
+      first_tile += __shfl_sync(0xffffffffu, s, 31);
+    }
+  }
+  if (tile0 >= tile1) {
+    if (is_pre) {   // an empty split still has its slot
+      for (int r = tid; r < MT * 16; r += WARPS * 32) {
+        const int rr = rt * MT * 16 + r;
+        if (rr < p.B * SG) {
+          float* ml = p.pre_ml + (((long long)n * p.n_split + c) * p.B * SG + rr) * 2;
+          ml[0] = -INFINITY, ml[1] = 0.f;
+        }
+      }
+    }
+    return;
+  }
+
+  const uint32_t ring = smem_u32(body) + warp * F::RING;
+  while (tile0 < tile1) {   // pieces
+    const KvView& kv = is_pre ? p.pre : p.own;
+    int key_lo, key_end, tb, te;   // key of tile 0 of the piece's sequence, end of its keys, tiles [tb, te) of it
+    if (is_pre) {
+      key_lo = p.pre_lo, key_end = p.P, tb = tile0, te = tile1;
+    } else {
+      len = len_of(p, b, false), cnt = count_of(p, b, len, false);
+      const int nt = tiles_of(p, len, cnt);
+      if (nt == 0) {
+        ++b;
+        continue;
+      }
+      key_lo = own_lo(p, len, cnt), key_end = len;
+      tb = tile0 - first_tile, te = min(nt, tile1 - first_tile);
+    }
+    const uint8_t* kbase = kv.k + b * kv.kb + n * kv.kn;
+    const uint8_t* vbase = kv.v + b * kv.vb + n * kv.vn;
+    const int8_t* kebase = Q8 ? kv.ke + b * kv.keb + n * kv.ken : nullptr;
+    const int8_t* vebase = Q8 ? kv.ve + b * kv.veb + n * kv.ven : nullptr;
+
+    // tile tb + warp + 4 j of the piece is this warp's j-th
+    const int mine = max(0, (te - tb - warp + WARPS - 1) / WARPS);
+    auto load = [&](int j) {
+      const int key0 = key_lo + (tb + warp + WARPS * j) * KB;
+      const uint32_t kd = ring + (j % F::ST) * 2 * F::TILE, vd = kd + F::TILE;
+#pragma unroll
+      for (int i = 0; i < KB * F::CPR / 32; ++i) {
+        const int x = i * 32 + lane, r = x / F::CPR, ch = x % F::CPR;
+        const bool in = key0 + r < key_end;
+        const long long key = in ? key0 + r : key_lo;
+        cp_async16(kd + tile_off<H, Q8>(r, ch), kbase + key * kv.ks + ch * 16, in);
+        cp_async16(vd + tile_off<H, Q8>(r, ch), vbase + key * kv.vs + ch * 16, in);
+      }
+    };
+    int ex_next = 0;   // this lane's key of the next tile: key exponent in the low byte, value exponent above
+    auto load_exps = [&](int j) {
+      const int key = key_lo + (tb + warp + WARPS * j) * KB + lane;
+      int ke = 0, ve = -128;
+      if (j < mine && key < key_end) ke = kebase[key * kv.kes], ve = vebase[key * kv.ves];
+      ex_next = (ke & 0xff) | (ve << 8);
+    };
+#pragma unroll
+    for (int j = 0; j < F::ST - 1; ++j) {
+      if (j < mine) load(j);
+      cp_async_commit();
+    }
+    if constexpr (Q8) load_exps(0);
+
+    // query fragments, each warp one 16-row tile
+    for (int mt = warp; mt < MT; mt += WARPS) {
+      const __nv_bfloat16* qrow[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int rr = (rt * MT + mt) * 16 + g + 8 * hf;
+        const int qb = is_pre ? rr / SG : b, ri = is_pre ? rr % SG : rr;
+        const bool in = is_pre ? rr < p.B * SG : rr < SG;
+        qrow[hf] = in ? p.q + qb * p.qb + (ri / p.G) * p.qs + (long long)(n * p.G + ri % p.G) * p.qh : nullptr;
+      }
+      if constexpr (!Q8) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          uint32_t w[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            w[x] = qrow[x & 1] ? *reinterpret_cast<const uint32_t*>(qrow[x & 1] + 16 * s + 2 * t + 8 * (x >> 1)) : 0u;
+          sQ[(mt * KS + s) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (t == 0) {
+          sScale[mt * 16 + g] = p.sl2;
+          sScale[mt * 16 + g + 8] = p.sl2;
+        }
+      } else {
+        uint2 w[2][KS];   // 4 consecutive channels per k step
+        float sc[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          float amax = 0.f;
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const int h0 = H == 32 ? t * 8 + 4 * s : 64 * (s / 4) + t * 16 + 4 * (s % 4);
+            w[hf][s] = qrow[hf] ? *reinterpret_cast<const uint2*>(qrow[hf] + h0) : make_uint2(0, 0);
+            const float f[4] = {__uint_as_float(w[hf][s].x << 16), __uint_as_float(w[hf][s].x & 0xffff0000u),
+                                __uint_as_float(w[hf][s].y << 16), __uint_as_float(w[hf][s].y & 0xffff0000u)};
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (fabsf(f[x]) < INFINITY) amax = fmaxf(amax, fabsf(f[x]));
+          }
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          const int e = max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -100);
+          sc[hf] = pow2c(-e);
+          if (t == 0) sScale[mt * 16 + g + 8 * hf] = pow2c(e) * p.sl2;
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          uint32_t a[2][2];
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            a[hf][0] = pack_f16x2(__uint_as_float(w[hf][s].x << 16) * sc[hf], __uint_as_float(w[hf][s].x & 0xffff0000u) * sc[hf]);
+            a[hf][1] = pack_f16x2(__uint_as_float(w[hf][s].y << 16) * sc[hf], __uint_as_float(w[hf][s].y & 0xffff0000u) * sc[hf]);
+          }
+          sQ[(mt * KS + s) * 32 + lane] = make_uint4(a[0][0], a[1][0], a[0][1], a[1][1]);
+        }
+      }
+    }
+    __syncthreads();
+
+    // visible keys [lo, hi) of this thread's rows; rows that are not there see all
+    int lo[MT][2], hi[MT][2], max_lo = 0, min_hi = key_end;
+    float qsc[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int rr = (rt * MT + mt) * 16 + g + 8 * hf;
+        lo[mt][hf] = 0, hi[mt][hf] = key_end;
+        qsc[mt][hf] = sScale[mt * 16 + g + 8 * hf];
+        if (is_pre) {
+          if (p.W > 0 && rr < p.B * SG) {
+            const int qb = rr / SG, ql = len_of(p, qb, false), qc = count_of(p, qb, ql, false), i = rr % SG / p.G;
+            if (i < qc) lo[mt][hf] = max(0, p.P + ql - qc + i - p.W + 1);
+          }
+        } else {
+          const int i = rr / p.G;
+          if (i < cnt) {
+            hi[mt][hf] = len - cnt + i + 1;
+            if (p.W > 0) lo[mt][hf] = max(0, len - cnt + i - p.W + 1);
+          }
+        }
+        max_lo = max(max_lo, lo[mt][hf]), min_hi = min(min_hi, hi[mt][hf]);
+      }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      max_lo = max(max_lo, __shfl_xor_sync(0xffffffffu, max_lo, o));
+      min_hi = min(min_hi, __shfl_xor_sync(0xffffffffu, min_hi, o));
+    }
+
+    float O[MT][JN][4], m[MT][2], l[MT][2], mo[MT][2];   // O in units of 2^mo (quantised) or 2^m
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int j = 0; j < JN; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) O[mt][j][x] = 0.f;
+      m[mt][0] = m[mt][1] = mo[mt][0] = mo[mt][1] = -INFINITY;
+      l[mt][0] = l[mt][1] = 0.f;
+    }
+
+    for (int j = 0; j < mine; ++j) {
+      cp_async_wait<F::ST - 2>();
+      __syncwarp();   // every lane's part of tile j has landed; tile j - 1 has been read
+      if (j + F::ST - 1 < mine) load(j + F::ST - 1);
+      cp_async_commit();
+      const int ex = ex_next;
+      if constexpr (Q8) load_exps(j + 1);
+      const uint32_t kt = ring + (j % F::ST) * 2 * F::TILE, vt = kt + F::TILE;
+      const int key0 = key_lo + (tb + warp + WARPS * j) * KB;
+
+      float s[MT][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[mt][i][x] = 0.f;
+      if constexpr (!Q8) {
+#pragma unroll
+        for (int k2 = 0; k2 < KS; k2 += 2) {
+          uint4 a[MT][2];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) a[mt][0] = sQ[(mt * KS + k2) * 32 + lane], a[mt][1] = sQ[(mt * KS + k2 + 1) * 32 + lane];
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            uint32_t r[4];
+            ldmatrix_x4(r, kt + tile_off<H, Q8>(8 * i + (lane & 7), 2 * k2 + (lane >> 3)));
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma_bf16(s[mt][i], a[mt][0], r[0], r[1]);
+              mma_bf16(s[mt][i], a[mt][1], r[2], r[3]);
+            }
+          }
+        }
+      } else {
+        constexpr int HS = H == 32 ? 2 : 4;   // k steps per lane's contiguous run of a row
+#pragma unroll
+        for (int k4 = 0; k4 < KS; k4 += HS) {
+          uint4 a[MT][HS];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int x = 0; x < HS; ++x) a[mt][x] = sQ[(mt * KS + k4 + x) * 32 + lane];
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            uint32_t w[4];
+            if constexpr (H == 32) {
+              asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1])
+                           : "r"(kt + (8 * i + g) * F::RB + t * 8) : "memory");
+            } else {
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                           : "r"(kt + tile_off<H, Q8>(8 * i + g, k4 + t)) : "memory");
+            }
+#pragma unroll
+            for (int x = 0; x < HS; ++x) {
+              const uint32_t b0 = e4m3x2_to_f16x2(w[x]), b1 = e4m3x2_to_f16x2(w[x] >> 16);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) mma_f16(s[mt][i], a[mt][x], b0, b1);
+            }
+          }
+        }
+      }
+
+      // scores in the log2 domain; masked ones minus infinity
+      const bool edge = key0 < max_lo || key0 + KB > min_hi;
+      int ekv[NT][2];
+      if constexpr (Q8) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) ekv[i][x] = __shfl_sync(0xffffffffu, ex, 8 * i + 2 * t + x);
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            float v = s[mt][i][x] * qsc[mt][x >> 1];
+            if constexpr (Q8) v *= pow2c((int)(int8_t)(ekv[i][x & 1] & 0xff));
+            const int key = key0 + 8 * i + 2 * t + (x & 1);
+            if (edge && (key < lo[mt][x >> 1] || key >= hi[mt][x >> 1])) v = -INFINITY;
+            s[mt][i][x] = v;
+          }
+      float wv[NT][2], ev[NT][2];   // 2^e and e of the value rows
+      if constexpr (Q8) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int e = ekv[i][x] >> 8;
+            ev[i][x] = (float)e;
+            wv[i][x] = pow2c(e);
+          }
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        // new maxima: m of the scores, mo of the scores plus value exponents (O's unit)
+        float mx[2] = {m[mt][0], m[mt][1]}, ox[2] = {mo[mt][0], mo[mt][1]};
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            mx[hf] = fmaxf(mx[hf], fmaxf(s[mt][i][2 * hf], s[mt][i][2 * hf + 1]));
+            if constexpr (Q8)
+              ox[hf] = fmaxf(ox[hf], fmaxf(s[mt][i][2 * hf] + ev[i][0], s[mt][i][2 * hf + 1] + ev[i][1]));
+          }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
+          if constexpr (Q8) {
+            ox[hf] = fmaxf(ox[hf], __shfl_xor_sync(0xffffffffu, ox[hf], 1));
+            ox[hf] = fmaxf(ox[hf], __shfl_xor_sync(0xffffffffu, ox[hf], 2));
+          } else {
+            ox[hf] = mx[hf];
+          }
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m[mt][0] || mx[1] > m[mt][1] || ox[0] > mo[mt][0] || ox[1] > mo[mt][1])) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const float al = mx[hf] == -INFINITY ? 1.f : ex2f(m[mt][hf] - mx[hf]);
+            const float ao = !Q8 ? al : ox[hf] == -INFINITY ? 1.f : ex2f(mo[mt][hf] - ox[hf]);
+            m[mt][hf] = mx[hf], mo[mt][hf] = ox[hf];
+            l[mt][hf] *= al;
+#pragma unroll
+            for (int jn = 0; jn < JN; ++jn) {
+              O[mt][jn][2 * hf] *= ao;
+              O[mt][jn][2 * hf + 1] *= ao;
+            }
+          }
+        }
+        float m0[2], r[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          m0[hf] = m[mt][hf] == -INFINITY ? 0.f : m[mt][hf];
+          if constexpr (Q8) r[hf] = m[mt][hf] == -INFINITY ? 0.f : ex2f(m[mt][hf] - mo[mt][hf]);
+        }
+        // weights -> A fragments of 16 keys each, kept where the scores were
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          float x0 = ex2f(s[mt][i][0] - m0[0]), x1 = ex2f(s[mt][i][1] - m0[0]);
+          float x2 = ex2f(s[mt][i][2] - m0[1]), x3 = ex2f(s[mt][i][3] - m0[1]);
+          l[mt][0] += x0 + x1;
+          l[mt][1] += x2 + x3;
+          uint32_t r0, r1;
+          if constexpr (Q8) {
+            r0 = pack_f16x2(x0 * r[0] * wv[i][0], x1 * r[0] * wv[i][1]);
+            r1 = pack_f16x2(x2 * r[1] * wv[i][0], x3 * r[1] * wv[i][1]);
+          } else {
+            r0 = pack_bf16x2(x0, x1);
+            r1 = pack_bf16x2(x2, x3);
+          }
+          s[mt][i][0] = __uint_as_float(r0), s[mt][i][1] = __uint_as_float(r1);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < KB / 16; ++k) {
+        uint4 a[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          a[mt] = make_uint4(__float_as_uint(s[mt][2 * k][0]), __float_as_uint(s[mt][2 * k][1]),
+                             __float_as_uint(s[mt][2 * k + 1][0]), __float_as_uint(s[mt][2 * k + 1][1]));
+        if constexpr (!Q8) {
+#pragma unroll
+          for (int jn = 0; jn < JN; jn += 2) {
+            uint32_t r[4];
+            ldmatrix_x4_trans(r, vt + tile_off<H, Q8>(16 * k + (lane & 15), jn + (lane >> 4)));
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma_bf16(O[mt][jn], a[mt], r[0], r[1]);
+              mma_bf16(O[mt][jn + 1], a[mt], r[2], r[3]);
+            }
+          }
+        } else {
+          // column n of output tile jn is channel n * (H / 8) + jn, so a lane's
+          // bytes of a value row are contiguous
+          constexpr int WN = H / 32;   // 4-byte words of a lane per row
+          uint32_t w[4][WN];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int r = 16 * k + 2 * t + (x & 1) + 8 * (x >> 1);
+            const uint32_t at = vt + tile_off<H, Q8>(r, g * (H / 8) / 16) + (g * (H / 8) & 15);
+            if constexpr (WN == 1) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[x][0]) : "r"(at) : "memory");
+            else if constexpr (WN == 2)
+              asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[x][0]), "=r"(w[x][1]) : "r"(at) : "memory");
+            else
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(w[x][0]), "=r"(w[x][1]), "=r"(w[x][2]), "=r"(w[x][3]) : "r"(at) : "memory");
+          }
+#pragma unroll
+          for (int y = 0; y < WN; ++y)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const uint32_t sel = z ? 0x7362u : 0x5140u;
+              const uint32_t p0 = __byte_perm(w[0][y], w[1][y], sel), p1 = __byte_perm(w[2][y], w[3][y], sel);
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const uint32_t b0 = e4m3x2_to_f16x2(p0 >> (16 * x)), b1 = e4m3x2_to_f16x2(p1 >> (16 * x));
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) mma_f16(O[mt][4 * y + 2 * z + x], a[mt], b0, b1);
+              }
+            }
+        }
+      }
+    }
+    cp_async_wait<0>();
+
+    // merge the warps: per row M = max m, weights 2^{m - M} (and 2^E)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        l[mt][hf] += __shfl_xor_sync(0xffffffffu, l[mt][hf], 1);
+        l[mt][hf] += __shfl_xor_sync(0xffffffffu, l[mt][hf], 2);
+      }
+    __syncthreads();   // every warp is done with its ring
+    constexpr int LD = H + 4;
+    float* sO = reinterpret_cast<float*>(body) + warp * MT * 16 * LD;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        float* row = sO + (mt * 16 + g + 8 * hf) * LD;
+        const float eO = Q8 && m[mt][hf] > -INFINITY ? ex2f(mo[mt][hf] - m[mt][hf]) : 1.f;
+#pragma unroll
+        for (int jn = 0; jn < JN; ++jn) {
+          const float x0 = O[mt][jn][2 * hf] * eO, x1 = O[mt][jn][2 * hf + 1] * eO;
+          if constexpr (!Q8) {
+            *reinterpret_cast<float2*>(row + 8 * jn + 2 * t) = make_float2(x0, x1);
+          } else {
+            row[2 * t * (H / 8) + jn] = x0;
+            row[(2 * t + 1) * (H / 8) + jn] = x1;
+          }
+        }
+        if (t == 0) row[H] = m[mt][hf], row[H + 1] = l[mt][hf];
+      }
+    __syncthreads();
+    constexpr int CL = H / 4;   // lanes per row
+    for (int x = tid; x < MT * 16 * CL; x += WARPS * 32) {
+      const int r = x / CL, ch = x % CL * 4, rr = rt * MT * 16 + r;
+      if (rr >= (is_pre ? p.B * SG : SG)) continue;
+      const float* row = reinterpret_cast<const float*>(body) + r * LD;
+      float M = -INFINITY, wt[WARPS], lsum = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, row[w * MT * 16 * LD + H]);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (M > -INFINITY)
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          wt[w] = ex2f(row[w * MT * 16 * LD + H] - M);
+          lsum += wt[w] * row[w * MT * 16 * LD + H + 1];
+          const float4 v = *reinterpret_cast<const float4*>(row + w * MT * 16 * LD + ch);
+          o.x += wt[w] * v.x, o.y += wt[w] * v.y, o.z += wt[w] * v.z, o.w += wt[w] * v.w;
+        }
+      const long long at = is_pre ? ((long long)n * p.n_split + c) * p.B * SG + rr
+                                  : ((long long)n * (p.n_suf + p.B) + c + b) * SG + rr;
+      *reinterpret_cast<float4*>((is_pre ? p.pre_o : p.own_o) + at * H + ch) = o;
+      if (ch == 0) *reinterpret_cast<float2*>((is_pre ? p.pre_ml : p.own_ml) + at * 2) = make_float2(M, lsum);
+    }
+    if (is_pre) break;
+    tile0 = first_tile + te;
+    if (tile0 < tile1) {   // the next sequence
+      first_tile = tile0;
+      ++b;
+      __syncthreads();
+    }
+  }
+}
+
+// Joins the pieces of one output row (b, i, h); WPR warps per row share them.
+template <int H, int WPR>
+__global__ void __launch_bounds__(128) decode_combine_kernel(const AttnParams p) {
+  constexpr int CL = H / 4, PPW = 32 / CL;   // lanes per piece, pieces per warp at a time
+  __shared__ float sm[4];
+  __shared__ float so[4][H + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row = (long long)blockIdx.x * (4 / WPR) + warp / WPR;
+  const int part = warp % WPR;
+  const long long rows = (long long)p.B * p.S * p.Nq;
+  const int SG = p.S * p.G;
+  bool live = row < rows;
+  int b = 0, i = 0, n = 0, g = 0, c_lo = 0, own_n = 0;
+  if (live) {
+    const int h = (int)(row % p.Nq);
+    const long long bs = row / p.Nq;
+    i = (int)(bs % p.S), b = (int)(bs / p.S);
+    n = h / p.G, g = h % p.G;
+    const int len = len_of(p, b, false);
+    live = i < count_of(p, b, len, false);
+    const int total = p.tile_start[p.B], per = max(WARPS, (total + p.n_suf - 1) / p.n_suf);
+    const int t0 = p.tile_start[b], t1 = p.tile_start[b + 1];
+    c_lo = t0 / per;
+    own_n = t1 > t0 ? (t1 - 1) / per - c_lo + 1 : 0;
+  }
+  const int np = live ? own_n + p.n_split : 0;
+  const long long own_at = ((long long)n * (p.n_suf + p.B) + c_lo + b) * SG + i * p.G + g;
+  const long long pre_at = (long long)n * p.n_split * p.B * SG + (long long)(b * p.S + i) * p.G + g;
+  auto slot = [&](int x) { return x < own_n ? own_at + (long long)x * SG : pre_at + (long long)(x - own_n) * p.B * SG; };
+  float M = -INFINITY;
+  for (int x = part * 32 + lane; x < np; x += WPR * 32) M = fmaxf(M, (x < own_n ? p.own_ml : p.pre_ml)[slot(x) * 2]);
+  M = warp_max(M);
+  if constexpr (WPR > 1) {
+    if (lane == 0) sm[warp] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  }
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  if (M > -INFINITY)
+#pragma unroll 4
+    for (int x = part * PPW + lane / CL; x < np; x += WPR * PPW) {
+      const bool own = x < own_n;
+      const long long at = slot(x);
+      const float2 ml = *reinterpret_cast<const float2*>((own ? p.own_ml : p.pre_ml) + at * 2);
+      const float4 v = *reinterpret_cast<const float4*>((own ? p.own_o : p.pre_o) + at * H + lane % CL * 4);
+      const float w = ex2f(ml.x - M);
+      // a piece that saw no key of this row has weight 0 and whatever O
+      if (w > 0.f) {
+        l += w * ml.y;
+        o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
+      }
+    }
+#pragma unroll
+  for (int d = CL; d < 32; d <<= 1) {
+    l += __shfl_xor_sync(0xffffffffu, l, d);
+    o.x += __shfl_xor_sync(0xffffffffu, o.x, d), o.y += __shfl_xor_sync(0xffffffffu, o.y, d);
+    o.z += __shfl_xor_sync(0xffffffffu, o.z, d), o.w += __shfl_xor_sync(0xffffffffu, o.w, d);
+  }
+  if constexpr (WPR > 1) {
+    if (lane < CL) {
+      float* d = so[warp] + lane * 4;
+      d[0] = o.x, d[1] = o.y, d[2] = o.z, d[3] = o.w;
+    }
+    if (lane == 0) so[warp][H] = l;
+    __syncthreads();
+    if (warp != 0) return;
+    l = so[0][H] + so[1][H] + so[2][H] + so[3][H];
+    if (lane < CL) {
+      float f[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) f[x] = so[0][lane * 4 + x] + so[1][lane * 4 + x] + so[2][lane * 4 + x] + so[3][lane * 4 + x];
+      o = make_float4(f[0], f[1], f[2], f[3]);
+    }
+  }
+  if (row < rows && lane < CL) {
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    *reinterpret_cast<uint2*>(p.out + row * H + lane * 4) =
+        make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  }
+}
+
+template <int H, bool Q8, int MT>
+void launch_attn(const AttnParams& p) {
+  constexpr int smem = Cfg<H, Q8, MT>::SMEM;
+  static bool configured[64] = {};
+  int dev = 0;
+  HB_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!configured[dev & 63]) {
+    HB_CUDA_CHECK(cudaFuncSetAttribute(decode_attn_kernel<H, Q8, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    configured[dev & 63] = true;
+  }
+  const long long blocks = (long long)p.n_pre + (long long)p.n_suf * p.N * p.own_rt;
+  HB_CHECK(blocks < (1ll << 31), "decode_attention: too many tiles");
+  decode_attn_kernel<H, Q8, MT><<<(unsigned)blocks, WARPS * 32, smem, cur_stream()>>>(p);
+  HB_CUDA_CHECK(cudaGetLastError());
+}
+
+template <int H>
+void launch_combine(const AttnParams& p) {
+  const long long rows = (long long)p.B * p.S * p.Nq;
+  // few rows of many pieces: four warps a row
+  if (p.n_split + p.n_suf > 8 && rows <= 4096) decode_combine_kernel<H, 4><<<(unsigned)rows, 128, 0, cur_stream()>>>(p);
+  else decode_combine_kernel<H, 1><<<(unsigned)((rows + 3) / 4), 128, 0, cur_stream()>>>(p);
+  HB_CUDA_CHECK(cudaGetLastError());
+}
+
+KvView view_of(const torch::Tensor& k, const torch::Tensor& v, const c10::optional<torch::Tensor>& ke,
+               const c10::optional<torch::Tensor>& ve) {
+  KvView o{};
+  const long long es = k.element_size();
+  o.k = (const uint8_t*)k.data_ptr(), o.v = (const uint8_t*)v.data_ptr();
+  o.kb = k.stride(0) * es, o.ks = k.stride(1) * es, o.kn = k.stride(2) * es;
+  o.vb = v.stride(0) * es, o.vs = v.stride(1) * es, o.vn = v.stride(2) * es;
+  if (ke) {
+    o.ke = ke->data_ptr<int8_t>(), o.ve = ve->data_ptr<int8_t>();
+    o.keb = ke->stride(0), o.kes = ke->stride(1), o.ken = ke->stride(2);
+    o.veb = ve->stride(0), o.ves = ve->stride(1), o.ven = ve->stride(2);
+  }
+  return o;
+}
+
+}  // namespace
+
+// q [B, S, Nq, H] bf16, own caches [B, C, N, H], prefix caches [1, P, N, H] (or
+// none) -> out [B, S, Nq, H] bf16 contiguous.
+void decode_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::optional<torch::Tensor> k_exp,
+                      c10::optional<torch::Tensor> v_exp, c10::optional<torch::Tensor> pk,
+                      c10::optional<torch::Tensor> pv, c10::optional<torch::Tensor> pk_exp,
+                      c10::optional<torch::Tensor> pv_exp, torch::Tensor lengths, c10::optional<torch::Tensor> counts,
+                      int64_t window, double scale, torch::Tensor out) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int H = (int)q.size(3);
+  HB_CHECK(H == 32 || H == 64 || H == 128, "decode_attention: head dim 32, 64 or 128");
+  AttnParams p{};
+  p.B = (int)q.size(0), p.S = (int)q.size(1), p.Nq = (int)q.size(2), p.N = (int)k.size(2);
+  if (p.B == 0 || p.S == 0) return;
+  p.G = p.Nq / p.N, p.C = (int)k.size(1), p.P = pk ? (int)pk->size(1) : 0;
+  p.W = (int)window;
+  HB_CHECK((long long)p.P + p.C < (1ll << 30), "decode_attention: more than 2^30 keys");
+  HB_CHECK((long long)p.B * p.S * p.G < (1ll << 30), "decode_attention: more than 2^30 query rows");
+  p.q = (const __nv_bfloat16*)q.data_ptr();
+  p.qb = q.stride(0), p.qs = q.stride(1), p.qh = q.stride(2);
+  const bool q8 = k_exp.has_value();
+  p.own = view_of(k, v, k_exp, v_exp);
+  if (p.P) {
+    p.pre = view_of(*pk, *pv, pk_exp, pv_exp);
+    p.pre.kb = p.pre.vb = p.pre.keb = p.pre.veb = 0;
+  }
+  p.lengths = lengths.data_ptr<int>();
+  p.counts = counts ? counts->data_ptr<int>() : nullptr;
+  p.sl2 = (float)(scale * 1.4426950408889634);
+  p.out = (__nv_bfloat16*)out.data_ptr();
+  p.status = status_ptr();
+
+  const int SG = p.S * p.G, R = p.B * SG;
+  const int mt = SG > 16 || (p.P && R > 16) ? 2 : 1;
+  const int sms = num_sms();
+  p.own_rt = (SG + 16 * mt - 1) / (16 * mt);
+  // own keys: about two CTAs per SM, at least 8 tiles of the full capacity each
+  const long long cap_tiles = (long long)p.B * ((p.C + KB - 1) / KB);
+  p.n_suf = (int)std::max<long long>(1, std::min<long long>(2ll * sms / ((long long)p.N * p.own_rt), cap_tiles / 8));
+  if (p.P) {
+    p.pre_lo = p.W > 0 ? std::max(0, p.P - p.W + 1) : 0;
+    p.pre_rt = (R + 16 * mt - 1) / (16 * mt);
+    const int tiles = (p.P - p.pre_lo + KB - 1) / KB;
+    p.n_split = (int)std::max<long long>(1, std::min<long long>(2ll * sms / ((long long)p.N * p.pre_rt), tiles / 8));
+    p.n_pre = p.n_split * p.N * p.pre_rt;
+  }
+  // workspace: own slots, prefix slots, tile starts
+  const long long own_rows = (long long)p.N * (p.n_suf + p.B) * SG, pre_rows = (long long)p.N * p.n_split * R;
+  torch::Tensor ws = torch::empty({(own_rows + pre_rows) * (H + 2) + p.B + 1}, q.options().dtype(torch::kFloat));
+  p.own_o = ws.data_ptr<float>();
+  p.pre_o = p.own_o + own_rows * H;
+  p.own_ml = p.pre_o + pre_rows * H;
+  p.pre_ml = p.own_ml + own_rows * 2;
+  p.tile_start = reinterpret_cast<int*>(p.pre_ml + pre_rows * 2);
+#define HB_ATTN(HH)                                                               \
+  do {                                                                            \
+    if (q8) mt == 2 ? launch_attn<HH, true, 2>(p) : launch_attn<HH, true, 1>(p);  \
+    else mt == 2 ? launch_attn<HH, false, 2>(p) : launch_attn<HH, false, 1>(p);   \
+    launch_combine<HH>(p);                                                        \
+  } while (0)
+  if (H == 32) HB_ATTN(32);
+  else if (H == 64) HB_ATTN(64);
+  else HB_ATTN(128);
+#undef HB_ATTN
+}
+
+}  // namespace hb

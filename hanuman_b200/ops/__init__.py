@@ -20,6 +20,7 @@ import torch
 from . import reference as ref
 from ._ext import available as ext_available  # noqa: F401
 from ._ext import check_status, ext  # noqa: F401
+from .kv_cache import KVCache, new_kv_cache  # noqa: F401
 
 
 def on_gpu(t: torch.Tensor) -> bool:
@@ -78,6 +79,59 @@ def attention(q, k, v, window: int = 0, q_offset: int = 0):
     return ref.causal_attention(q, k, v, window, q_offset=q_offset)
 
 
+# ------------------------------------------------------------------ cached decoding
+def kv_cache_write(cache: KVCache, k, v, starts, counts=None) -> None:
+    """Write keys and values ``k, v [B, S, Nkv, H]`` (bf16 or fp32; any strides
+    of whole rows) into rows ``starts[b] + i`` of ``cache``, ``i < counts[b]``
+    (all S without ``counts``), quantising them if the cache is quantised: one
+    power-of-two exponent per row, e4m3 codes rounded to nearest even,
+    infinities saturated, NaN kept.  ``starts`` / ``counts``: whole numbers [B]
+    on the device, or one int for all.  On the GPU a row outside the cache is
+    skipped and recorded in the status word."""
+    from .kv_cache import kv_cache_write as f
+    f(cache, k, v, starts, counts)
+
+
+def kv_cache_read(cache: KVCache, starts, n: int):
+    """Rows ``starts[b] .. starts[b] + n - 1`` of every sequence as values
+    ``(k, v) [B, n, Nkv, H]`` (bf16 on the GPU, exact for either cache type)."""
+    from .kv_cache import kv_cache_read as f
+    return f(cache, starts, n)
+
+
+def decode_attention(q, cache: KVCache, lengths, counts=None, prefix: Optional[KVCache] = None, window: int = 0,
+                     scale: Optional[float] = None):
+    """Attention of the newest tokens over cached keys and values.
+
+    ``q [B, S, Nq, H]``: query i of sequence b, ``i < counts[b]`` (all S without
+    ``counts``), is its token ``lengths[b] - counts[b] + i``; ``lengths [B]``
+    counts a sequence's rows in ``cache``, the new ones included.  ``prefix``
+    (one sequence, ``[1, P, Nkv, H]``) holds P earlier tokens that all sequences
+    share; its keys are read once for the whole batch.  Causal, with an optional
+    window counted over prefix and own tokens.  Returns ``[B, S, Nq, H]`` in q's
+    type; queries past ``counts`` give 0."""
+    from .kv_cache import decode_attention as f
+    return f(q, cache, lengths, counts, prefix, window, scale)
+
+
+def verify_draft(target_logits, draft_tokens, uniform, noise, draft_logits=None, draft_lens=None, temperature=1.0):
+    """Accept drafted tokens by rejection sampling and draw the next token.
+
+    ``target_logits [B, K + 1, V]`` (fp32 or bf16), ``draft_tokens [B, K]``,
+    ``draft_logits [B, K, V]`` or None for a draft that is certain of its
+    tokens, ``draft_lens [B]`` drafted tokens that count (all K by default),
+    ``temperature`` a number or ``[B]`` fp32 (0: greedy).  Random numbers are
+    inputs: ``uniform [B, K]`` in [0, 1) for the acceptance and ``noise [B, V]``
+    > 0, exponentially distributed, for the draw (argmax of p / noise).
+
+    Returns ``tokens [B, K + 1]`` (accepted drafts, the next token, then -1),
+    ``accepted [B]`` and ``logp [B, K + 1]``, the log probability of each
+    emitted token under the target at that temperature (0 where greedy).  NaN
+    logits count as minus infinity; a row with none left yields token -1."""
+    from .spec import verify_draft as f
+    return f(target_logits, draft_tokens, uniform, noise, draft_logits, draft_lens, temperature)
+
+
 # ------------------------------------------------------------------ swiglu
 def swiglu_act(gu: torch.Tensor) -> torch.Tensor:
     """``silu(g) * u`` for ``gu = [g | u]`` along the last axis."""
@@ -101,6 +155,21 @@ def kda_core(q, k, v, g, beta, scale: float, chunk: int, recompute: bool = False
                           use_reentrant=False)
     o, _ = ref.kda_chunked(q, k, v, g, beta, scale, chunk)
     return o
+
+
+def kda_recurrent(q, k, v, g, beta, scale: Optional[float] = None, state: Optional[torch.Tensor] = None,
+                  counts=None):
+    """Gated delta rule token by token from a carried state: one decoding step
+    (S = 1), a few drafted tokens, or a prompt.
+
+    ``q, k, v [B, S, H, K]`` (fp32 or bf16), ``g`` like them and ``beta
+    [B, S, H]`` fp32; ``state [B, H, K, K]`` fp32 (``[1, H, K, K]``: one state
+    that all sequences start from; None: zeros).  Only the first ``counts[b]``
+    tokens of a sequence are applied (all S without it); later ones give 0.
+    Returns ``(o [B, S, H, K] fp32, new state [B, H, K, K] fp32)``; ``state``
+    itself is left as it is."""
+    from .kda import kda_recurrent as f
+    return f(q, k, v, g, beta, scale, state, counts)
 
 
 # ------------------------------------------------------------------ loss

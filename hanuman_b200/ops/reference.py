@@ -236,6 +236,187 @@ def kda_chunked(q, k, v, g, beta, scale: Optional[float] = None, chunk: int = 64
     return torch.cat(outs, dim=1), st
 
 
+def kda_recurrent_ragged(q, k, v, g, beta, scale: Optional[float] = None,
+                         state: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None):
+    """:func:`kda_recurrent` of ragged batches: tokens at ``t >= counts[b]``
+    leave the state as it is and give 0; ``state [1, H, K, V]`` is shared."""
+    B, S, H, K = q.shape
+    if state is not None:
+        state = state.expand(B, *state.shape[1:])
+    if S == 0:
+        st = torch.zeros(B, H, K, v.shape[-1], device=q.device) if state is None else state.clone()
+        return q.new_zeros(B, 0, H, v.shape[-1], dtype=torch.float32), st
+    if counts is None:
+        return kda_recurrent(q, k, v, g, beta, scale, state)
+    live = torch.arange(S, device=q.device) < counts[:, None]
+    off = ~live[:, :, None, None]
+    zero = lambda x: x.masked_fill(off, 0)   # no decay, no write: the token changes nothing
+    o, st = kda_recurrent(zero(q), zero(k), zero(v), zero(g), beta.masked_fill(off[..., 0], 0), scale, state)
+    return o, st
+
+
+# ---------------------------------------------------------------------------
+# Cached decoding
+# ---------------------------------------------------------------------------
+def exact_pow2(e: torch.Tensor) -> torch.Tensor:
+    """2^e in fp32, exactly, for whole -126 <= e <= 127."""
+    return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def quantise_rows(x: torch.Tensor):
+    """Rows (last axis) as e4m3 codes and int8 exponents: the least e with
+    ``amax <= 448 * 2^e`` (amax over finite values, e in [-120, 119], 0 for a
+    zero row), codes of ``x * 2^-e`` rounded to nearest even and saturated."""
+    x = x.float()
+    amax = x.abs().masked_fill(~torch.isfinite(x), 0).amax(-1)
+    m, e = torch.frexp(amax)                       # amax = m 2^e, m in [0.5, 1); 448 = 0.875 * 2^9
+    e = (e - 9 + (m > 0.875).to(e.dtype)).clamp(-120, 119)
+    e = e.masked_fill(amax == 0, 0)
+    y = (x * exact_pow2(-e)[..., None]).clamp(-448.0, 448.0)
+    return y.to(torch.float8_e4m3fn), e.to(torch.int8)
+
+
+def dequantise_rows(code: torch.Tensor, e: torch.Tensor) -> torch.Tensor:
+    return code.float() * exact_pow2(e)[..., None]
+
+
+def _cache_rows(cache, starts, n):
+    pos = starts[:, None].long() + torch.arange(n, device=starts.device)
+    return torch.arange(pos.shape[0], device=starts.device)[:, None], pos
+
+
+def kv_cache_write(cache, k, v, starts, counts=None):
+    B, S = k.shape[:2]
+    rows, pos = _cache_rows(cache, starts, S)
+    live = torch.ones(B, S, dtype=torch.bool, device=k.device) if counts is None else \
+        torch.arange(S, device=k.device) < counts[:, None]
+    if bool((live & ((pos < 0) | (pos >= cache.k.shape[1]))).any()):
+        raise IndexError("kv_cache_write: a row outside the cache")
+    b, i = live.nonzero(as_tuple=True)
+    for x, c, e in ((k, cache.k, cache.k_exp), (v, cache.v, cache.v_exp)):
+        if e is None:
+            c[b, pos[b, i]] = x[b, i].to(c.dtype)
+        else:
+            y, ye = quantise_rows(x[b, i])
+            c.view(torch.uint8)[b, pos[b, i]] = y.view(torch.uint8)
+            e[b, pos[b, i]] = ye
+
+
+def cache_values(cache):
+    """Every row of a cache as values (fp32 for quantised caches)."""
+    if cache.k_exp is None:
+        return cache.k, cache.v
+    return dequantise_rows(cache.k, cache.k_exp), dequantise_rows(cache.v, cache.v_exp)
+
+
+def kv_cache_read(cache, starts, n: int):
+    rows, pos = _cache_rows(cache, starts, n)
+    if n and bool(((pos < 0) | (pos >= cache.k.shape[1])).any()):
+        raise IndexError("kv_cache_read: a row outside the cache")
+    k, v = (t[rows, pos] for t in cache_values(cache))
+    return (k, v) if cache.k_exp is None else (k.bfloat16(), v.bfloat16())
+
+
+def decode_attention(q, cache, lengths, counts=None, prefix=None, window: int = 0, scale: Optional[float] = None):
+    """Query (b, i), i < counts[b], at position ``P + lengths[b] - counts[b] + i``
+    over the shared prefix (keys at 0 .. P - 1) and its own rows (at P + j)."""
+    B, S, Nq, H = q.shape
+    N = cache.k.shape[2]
+    scale = (1.0 / math.sqrt(H)) if scale is None else scale
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    k, v = (t.to(wide) for t in cache_values(cache))
+    P = 0
+    if prefix is not None:
+        P = prefix.k.shape[1]
+        pk, pv = (t.to(wide).expand(B, -1, -1, -1) for t in cache_values(prefix))
+        k, v = torch.cat([pk, k], 1), torch.cat([pv, v], 1)
+    lengths = lengths.long().clamp(0, cache.k.shape[1])
+    counts = lengths.clamp(max=S) if counts is None else torch.minimum(counts.long().clamp(0, S), lengths)
+    step = torch.arange(S, device=q.device)
+    live = step < counts[:, None]
+    pos = P + (lengths - counts)[:, None] + step
+    kp = torch.arange(k.shape[1], device=q.device)
+    seen = live[..., None] & (kp <= pos[..., None])
+    if window > 0:
+        seen = seen & (pos[..., None] - kp < window)
+    s = torch.einsum("bsngh,bcnh->bnsgc", q.to(wide).view(B, S, N, Nq // N, H), k) * scale
+    s = s.masked_fill(~seen[:, None, :, None, :], float("-inf"))
+    p = torch.softmax(s, -1).masked_fill(~live[:, None, :, None, None], 0)
+    # rows that nothing can see are not read: whatever they hold, weight 0 gives 0
+    v = v.masked_fill(~seen.any(1)[:, :, None, None], 0)
+    o = torch.einsum("bnsgc,bcnh->bsngh", p, v)
+    return o.reshape(B, S, Nq, H).to(q.dtype)
+
+
+def verify_draft(target, tokens, uniform, noise, draft=None, lens=None, temperature=None):
+    """Sequential restatement of speculative verification (one sequence and one
+    position at a time); see :func:`hanuman_b200.ops.verify_draft`."""
+    B, K1, V = target.shape
+    K = K1 - 1
+    dev = target.device
+    out = torch.full((B, K1), -1, dtype=torch.int64, device=dev)
+    accepted = torch.zeros(B, dtype=torch.int64, device=dev)
+    logp = torch.zeros(B, K1, dtype=torch.float32, device=dev)
+    wide = torch.float64 if target.dtype == torch.float64 else torch.float32
+
+    def clean(x):
+        x = x.to(wide)
+        return x.masked_fill(x.isnan(), float("-inf"))
+
+    def softmax(x, temp):
+        if bool((x == float("-inf")).all()):
+            return torch.zeros_like(x)
+        e = torch.exp((x - x.max()) / temp).masked_fill(x == x.max(), 1)
+        return e / e.sum()
+
+    for b in range(B):
+        temp = float(temperature[b])
+        L = K if lens is None else int(lens[b])
+        n = 0
+        while True:
+            t = clean(target[b, n])
+            empty = bool((t == float("-inf")).all())
+            if not temp > 0:
+                best = -1 if empty else int((t == t.max()).nonzero()[0, 0])
+                if n < L and int(tokens[b, n]) == best:
+                    out[b, n] = best
+                    n += 1
+                    continue
+                out[b, n] = best
+                break
+            p = softmax(t, temp)
+            x = int(tokens[b, n]) if n < L else -1
+            q = torch.zeros_like(p)
+            if n < L:
+                if draft is None:
+                    q[x] = 1
+                else:
+                    q = softmax(clean(draft[b, n]), temp)
+                if bool(uniform[b, n] * q[x] < p[x]):
+                    out[b, n] = x
+                    logp[b, n] = torch.log(p[x])
+                    n += 1
+                    continue
+                r = (p - q).clamp(min=0)
+                if draft is None:
+                    r = p.clone()
+                    r[x] = 0
+                if bool((r > 0).any()):
+                    p_draw = r
+                else:
+                    p_draw = p
+            else:
+                p_draw = p
+            if bool((p_draw > 0).any()):
+                score = p_draw / noise[b].to(wide)
+                j = int((score == score.max()).nonzero()[0, 0])
+                out[b, n] = j
+                logp[b, n] = torch.log(p[j])
+            break
+        accepted[b] = n
+    return out, accepted, logp
+
+
 # ---------------------------------------------------------------------------
 # MoE (model/moe.py)
 # ---------------------------------------------------------------------------
