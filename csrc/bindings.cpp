@@ -129,23 +129,21 @@ void ep_return(torch::Tensor rows, torch::Tensor cnt, torch::Tensor peers, int64
 void ep_combine(torch::Tensor ret, c10::optional<torch::Tensor> w, torch::Tensor topi, torch::Tensor pos,
                 torch::Tensor starts, torch::Tensor out, int64_t cap);
 // cached decoding
-void kv_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Tensor v_cache,
-                    c10::optional<torch::Tensor> k_exp, c10::optional<torch::Tensor> v_exp, torch::Tensor starts,
-                    c10::optional<torch::Tensor> counts);
-void kv_cache_read(torch::Tensor k_cache, torch::Tensor v_cache, c10::optional<torch::Tensor> k_exp,
-                   c10::optional<torch::Tensor> v_exp, torch::Tensor starts, torch::Tensor k_out,
-                   torch::Tensor v_out);
-void decode_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::optional<torch::Tensor> k_exp,
-                      c10::optional<torch::Tensor> v_exp, c10::optional<torch::Tensor> pk,
-                      c10::optional<torch::Tensor> pv, c10::optional<torch::Tensor> pk_exp,
-                      c10::optional<torch::Tensor> pv_exp, torch::Tensor lengths, c10::optional<torch::Tensor> counts,
-                      int64_t window, double scale, torch::Tensor out);
-void kda_recurrent(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor g, torch::Tensor beta, double scale,
-                   c10::optional<torch::Tensor> s0, c10::optional<torch::Tensor> counts, torch::Tensor o,
-                   torch::Tensor s1);
-void verify_draft(torch::Tensor target, c10::optional<torch::Tensor> draft, torch::Tensor tokens, torch::Tensor uniform,
-                  torch::Tensor noise, c10::optional<torch::Tensor> lens, c10::optional<torch::Tensor> temperature,
-                  double temp, torch::Tensor out, torch::Tensor accepted, torch::Tensor logp);
+using OptTensor = c10::optional<torch::Tensor>;
+void kv_cache_write(torch::Tensor k_cache, torch::Tensor v_cache, OptTensor k_exp, OptTensor v_exp, torch::Tensor k,
+                    torch::Tensor v, torch::Tensor starts, OptTensor counts);
+std::tuple<torch::Tensor, torch::Tensor> kv_cache_read(torch::Tensor k_cache, torch::Tensor v_cache, OptTensor k_exp,
+                                                       OptTensor v_exp, OptTensor starts, int64_t S);
+torch::Tensor decode_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, OptTensor k_exp, OptTensor v_exp,
+                               OptTensor pk, OptTensor pv, OptTensor pk_exp, OptTensor pv_exp, torch::Tensor lengths,
+                               OptTensor counts, int64_t window, c10::optional<double> scale);
+std::tuple<torch::Tensor, torch::Tensor> kda_recurrent(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor g,
+                                                       torch::Tensor beta, c10::optional<double> scale, OptTensor s0,
+                                                       OptTensor counts);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> verify_draft(torch::Tensor target, torch::Tensor tokens,
+                                                                     torch::Tensor uniform, torch::Tensor noise,
+                                                                     OptTensor draft, OptTensor lens,
+                                                                     OptTensor temperature, double temp);
 }  // namespace hb
 
 static int64_t read_status() {

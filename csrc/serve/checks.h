@@ -1,0 +1,56 @@
+// Argument checks of the decoding operators: a wrong argument raises ValueError.
+// They stand here and not in Python because a decoding step makes many small
+// calls, and the checks of one took longer there than its kernel (about 15 us of
+// Python against 1 us here).
+#pragma once
+#include "../common/host.h"
+
+namespace hb {
+
+inline void need(bool ok, const char* what) {
+  if (!ok) throw pybind11::value_error(what);
+}
+// These operators have no backward: refuse rather than cut the graph.
+inline bool wants_grad(const torch::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+// Rows readable in place: contiguous, at 16-byte multiples.
+inline bool rows_aligned(const torch::Tensor& t) {
+  const int64_t es = t.element_size(), d = t.dim();
+  if (t.stride(d - 1) != 1 && t.size(d - 1) > 1) return false;
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  for (int64_t i = 0; i + 1 < d; ++i)
+    if (t.size(i) > 1 && t.stride(i) * es % 16) return false;
+  return true;
+}
+// t, or an aligned copy (a view of contiguous values at an odd address too).
+inline torch::Tensor aligned_rows(const torch::Tensor& t) {
+  return rows_aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+using OptTensor = c10::optional<torch::Tensor>;
+
+// Whole numbers [B] as contiguous int32.
+inline torch::Tensor whole(const torch::Tensor& t, int64_t B, const torch::Device& dev, const char* what) {
+  need(t.dim() == 1 && t.size(0) == B && t.device() == dev && at::isIntegralType(t.scalar_type(), false), what);
+  return t.scalar_type() == at::kInt ? t.contiguous() : t.to(at::kInt).contiguous();
+}
+
+// A cache [B, C, N, H]: bf16, or e4m3 codes with int8 exponents [B, C, N].
+inline void check_cache(const torch::Tensor& k, const torch::Tensor& v, const OptTensor& ke, const OptTensor& ve,
+                        const torch::Device& dev) {
+  need(k.dim() == 4 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.device() == dev && v.device() == dev,
+       "cache: keys and values of one shape [B, C, N, H], type and device");
+  if (ke || ve) {
+    need(k.scalar_type() == at::kFloat8_e4m3fn, "cache: a cache with exponents holds float8_e4m3fn codes");
+    for (const OptTensor* e : {&ke, &ve})
+      need(*e && (*e)->scalar_type() == at::kChar && (*e)->sizes() == k.sizes().slice(0, 3) && (*e)->device() == dev,
+           "cache: int8 exponents [B, C, N] of keys and values");
+  } else {
+    need(k.scalar_type() == at::kBFloat16, "cache: bf16 rows, or float8_e4m3fn codes with their exponents");
+  }
+  const int64_t H = k.size(3);
+  need(H == 32 || H == 64 || H == 128, "cache: head dim 32, 64 or 128");
+  need(rows_aligned(k) && rows_aligned(v), "cache: contiguous rows at 16-byte multiples");
+}
+
+}  // namespace hb

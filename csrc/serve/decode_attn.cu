@@ -17,6 +17,10 @@
 // Prefix keys: the rows of all sequences (B * S * G of a KV head) are queries of
 // one long sequence: row tiles x key splits.
 //
+// When there are many sequences and none is long, a CTA takes all own keys of one
+// (sequence, KV head), joins the prefix pieces with its own result and writes the
+// output (WHOLE).
+//
 // A CTA is 4 warps that share the rows and take every fourth 32-key tile, each
 // with its own cp.async ring, m, l and O (no barrier between tiles); they merge
 // through shared memory at the end of a piece.  Products on mma.sync: at S * G
@@ -32,72 +36,56 @@
 #include <torch/extension.h>
 
 #include "../common/host.h"
+#include "attn_params.cuh"
+#include "checks.h"
 #include "mma.cuh"
 
 namespace hb {
+std::tuple<torch::Tensor, torch::Tensor> kv_cache_read(torch::Tensor k_cache, torch::Tensor v_cache, OptTensor k_exp,
+                                                       OptTensor v_exp, OptTensor starts, int64_t S);
 namespace {
 
 constexpr int WARPS = 4;
 constexpr int KB = 32;   // keys per warp tile
-constexpr float LOG2E_D = 1.4426950408889634f;
 
-struct KvView {
-  const uint8_t *k, *v;
-  const int8_t *ke, *ve;
-  long long kb, ks, kn, vb, vs, vn;          // bytes
-  long long keb, kes, ken, veb, ves, ven;    // elements
-};
-struct AttnParams {
-  const __nv_bfloat16* q;
-  long long qb, qs, qh;
-  KvView own, pre;
-  const int *lengths, *counts;
-  int B, S, Nq, N, G, C, P, W;
-  int pre_lo;                 // first prefix key that any query can see
-  float sl2;
-  int n_pre, n_split, pre_rt; // prefix CTAs; key splits; row tiles
-  int n_suf, own_rt;          // own-key CTAs per (KV head, row tile); row tiles of a sequence
-  float *own_o, *own_ml, *pre_o, *pre_ml;
-  int* tile_start;            // [B + 1]
-  __nv_bfloat16* out;         // [B, S, Nq, H] contiguous
-  int* status;
-};
-
-HB_DEVICE float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // 2^e for integers, 0 below the normal range.
 HB_DEVICE float pow2c(int e) { return e < -126 ? 0.f : __int_as_float((min(e, 127) + 127) << 23); }
 
-HB_DEVICE int len_of(const AttnParams& p, int b, bool report) {
-  const int x = p.lengths[b], y = min(max(x, 0), p.C);
-  if (report && x != y) set_error(p.status, kErrBounds);
-  return y;
-}
-HB_DEVICE int count_of(const AttnParams& p, int b, int len, bool report) {
-  if (!p.counts) return min(p.S, len);
-  const int x = p.counts[b], y = min(max(x, 0), min(p.S, len));
-  if (report && x != y) set_error(p.status, kErrBounds);
-  return y;
-}
 // First own key that any query of the sequence sees.
 HB_DEVICE int own_lo(const AttnParams& p, int len, int cnt) { return p.W > 0 ? max(0, len - cnt - p.W + 1) : 0; }
 HB_DEVICE int tiles_of(const AttnParams& p, int len, int cnt) {
   return cnt > 0 ? (len - own_lo(p, len, cnt) + KB - 1) / KB : 0;
 }
 
+// The prefix pieces of one row (of KV head n): how many, index of the first, and
+// rows from one piece to the next.
+struct PrePieces {
+  int n;
+  long long at, step;
+};
+HB_DEVICE PrePieces pre_pieces(const AttnParams& p, int n, int row) {
+  if (p.tc_ctas > 0) {
+    const int u = n * p.tc_rt + row / p.tc_rows;
+    const long long t0 = (long long)u * p.tc_tiles;
+    const int c0 = (int)(t0 / p.tc_per);
+    return {(int)((t0 + p.tc_tiles - 1) / p.tc_per) - c0 + 1, ((long long)c0 + u) * p.tc_rows + row % p.tc_rows, p.tc_rows};
+  }
+  const long long R = (long long)p.B * p.S * p.G;
+  return {p.n_split, (long long)n * p.n_split * R + row, R};
+}
+constexpr int MAX_PRE = 160;   // prefix pieces of a row
+
 template <int H, bool Q8, int MT>
 struct Cfg {
   static constexpr int RB = Q8 ? H : 2 * H;             // bytes of a cached row
   static constexpr int CPR = RB / 16;                   // 16-byte chunks of it
   static constexpr int TILE = KB * RB;                  // K or V tile
-  static constexpr int ST = RB >= 256 ? 3 : 4;          // ring stages
+  static constexpr int ST = Q8 ? 3 : 2;                 // ring stages
   static constexpr int RING = ST * 2 * TILE;            // per warp
   static constexpr int QF = MT * (H / 16) * 32 * 16;    // query fragments
   static constexpr int MERGE = WARPS * MT * 16 * (H + 4) * 4;
-  static constexpr int BODY = WARPS * RING > MERGE ? WARPS * RING : MERGE;
+  static constexpr int JOIN = MERGE + MT * 16 * MAX_PRE * 4;
+  static constexpr int BODY = WARPS * RING > JOIN ? WARPS * RING : JOIN;
   static constexpr int SMEM = QF + MT * 16 * 4 + BODY;
 };
 
@@ -112,7 +100,7 @@ HB_DEVICE int tile_off(int r, int c) {
   else return r * RB + (c << 4);
 }
 
-template <int H, bool Q8, int MT>
+template <int H, bool Q8, int MT, bool WHOLE>
 __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParams p) {
   using F = Cfg<H, Q8, MT>;
   constexpr int KS = H / 16;        // k16 steps of q.k
@@ -126,11 +114,17 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int SG = p.S * p.G;
-  const bool is_pre = (int)blockIdx.x < p.n_pre;
+  const bool is_pre = !WHOLE && (int)blockIdx.x < p.n_pre;
 
   int n, rt, b = 0, c = 0, tile0, tile1, first_tile = 0;   // tile range of this CTA; first tile of sequence b
   int len = 0, cnt = 0;
-  if (is_pre) {
+  if constexpr (WHOLE) {
+    int x = blockIdx.x;
+    rt = x % p.own_rt, x /= p.own_rt;
+    n = x % p.N, b = x / p.N;
+    len = len_of(p, b, n == 0 && rt == 0), cnt = count_of(p, b, len, n == 0 && rt == 0);
+    tile0 = 0, tile1 = tiles_of(p, len, cnt);
+  } else if (is_pre) {
     int x = blockIdx.x;
     rt = x % p.pre_rt, x /= p.pre_rt;
     n = x % p.N;
@@ -193,7 +187,7 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
       first_tile += __shfl_sync(0xffffffffu, s, 31);
     }
   }
-  if (tile0 >= tile1) {
+  if (!WHOLE && tile0 >= tile1) {
     if (is_pre) {   // an empty split still has its slot
       for (int r = tid; r < MT * 16; r += WARPS * 32) {
         const int rr = rt * MT * 16 + r;
@@ -207,11 +201,13 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
   }
 
   const uint32_t ring = smem_u32(body) + warp * F::RING;
-  while (tile0 < tile1) {   // pieces
+  while (WHOLE || tile0 < tile1) {   // pieces
     const KvView& kv = is_pre ? p.pre : p.own;
     int key_lo, key_end, tb, te;   // key of tile 0 of the piece's sequence, end of its keys, tiles [tb, te) of it
     if (is_pre) {
       key_lo = p.pre_lo, key_end = p.P, tb = tile0, te = tile1;
+    } else if constexpr (WHOLE) {
+      key_lo = own_lo(p, len, cnt), key_end = len, tb = 0, te = tile1;
     } else {
       len = len_of(p, b, false), cnt = count_of(p, b, len, false);
       const int nt = tiles_of(p, len, cnt);
@@ -595,6 +591,65 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
       }
     __syncthreads();
     constexpr int CL = H / 4;   // lanes per row
+    if constexpr (WHOLE) {
+      // all of the sequence's own keys are here: join them with the prefix pieces
+      wait_previous();
+      const int rows = min(SG - rt * MT * 16, MT * 16);
+      float* sW = reinterpret_cast<float*>(body) + WARPS * MT * 16 * LD;   // weights of the pieces, then 1 / l
+      // a warp per row: M over the warps and the prefix pieces, weights, 1 / l
+      for (int r = warp; r < rows; r += WARPS) {
+        const int rr = rt * MT * 16 + r;
+        const float* row = reinterpret_cast<const float*>(body) + r * LD;
+        const PrePieces pre = p.P > 0 ? pre_pieces(p, n, b * SG + rr) : PrePieces{0, 0, 0};
+        float M = lane < WARPS ? row[lane * MT * 16 * LD + H] : -INFINITY;
+        for (int x = lane; x < pre.n; x += 32) {
+          const float mp = p.pre_ml[(pre.at + x * pre.step) * 2];
+          M = fmaxf(M, mp);
+        }
+        M = warp_max(M);
+        float l = 0.f;
+        float* w = sW + r * MAX_PRE;
+        if (lane < WARPS) {
+          const float x = M > -INFINITY ? ex2f(row[lane * MT * 16 * LD + H] - M) : 0.f;
+          l = x * row[lane * MT * 16 * LD + H + 1];
+          w[lane] = x;
+        }
+        for (int x = lane; x < pre.n; x += 32) {
+          const float2 ml = *reinterpret_cast<const float2*>(p.pre_ml + (pre.at + x * pre.step) * 2);
+          const float e = M > -INFINITY ? ex2f(ml.x - M) : 0.f;
+          l += e * ml.y;
+          w[WARPS + x] = e;
+        }
+        l = warp_sum(l);
+        if (lane == 0) w[MAX_PRE - 1] = l > 0.f && rr / p.G < cnt ? 1.f / l : 0.f;
+      }
+      __syncthreads();
+      for (int x = tid; x < rows * CL; x += WARPS * 32) {
+        const int r = x / CL, ch = x % CL * 4, rr = rt * MT * 16 + r;
+        const float* row = reinterpret_cast<const float*>(body) + r * LD + ch;
+        const float* w = sW + r * MAX_PRE;
+        const float inv = w[MAX_PRE - 1];
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        const auto add = [&](float wt, const float4& v) {
+          if (wt > 0.f) o.x += wt * v.x, o.y += wt * v.y, o.z += wt * v.z, o.w += wt * v.w;
+        };
+        if (inv > 0.f) {
+#pragma unroll
+          for (int y = 0; y < WARPS; ++y) add(w[y], *reinterpret_cast<const float4*>(row + y * MT * 16 * LD));
+          if (p.P > 0) {
+            const PrePieces pre = pre_pieces(p, n, b * SG + rr);
+            const float4* src = reinterpret_cast<const float4*>(p.pre_o + pre.at * H + ch);
+            const long long step = pre.step * (H / 4);
+#pragma unroll 8
+            for (int y = 0; y < pre.n; ++y) add(w[WARPS + y], src[y * step]);
+          }
+        }
+        const int i = rr / p.G, h = n * p.G + rr % p.G;
+        *reinterpret_cast<uint2*>(p.out + (((long long)b * p.S + i) * p.Nq + h) * H + ch) =
+            make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+      }
+      break;
+    }
     for (int x = tid; x < MT * 16 * CL; x += WARPS * 32) {
       const int r = x / CL, ch = x % CL * 4, rr = rt * MT * 16 + r;
       if (rr >= (is_pre ? p.B * SG : SG)) continue;
@@ -651,10 +706,10 @@ __global__ void __launch_bounds__(128) decode_combine_kernel(const AttnParams p)
     c_lo = t0 / per;
     own_n = t1 > t0 ? (t1 - 1) / per - c_lo + 1 : 0;
   }
-  const int np = live ? own_n + p.n_split : 0;
+  const PrePieces pre = pre_pieces(p, n, (b * p.S + i) * p.G + g);
+  const int np = live ? own_n + pre.n : 0;
   const long long own_at = ((long long)n * (p.n_suf + p.B) + c_lo + b) * SG + i * p.G + g;
-  const long long pre_at = (long long)n * p.n_split * p.B * SG + (long long)(b * p.S + i) * p.G + g;
-  auto slot = [&](int x) { return x < own_n ? own_at + (long long)x * SG : pre_at + (long long)(x - own_n) * p.B * SG; };
+  auto slot = [&](int x) { return x < own_n ? own_at + (long long)x * SG : pre.at + (x - own_n) * pre.step; };
   float M = -INFINITY;
   for (int x = part * 32 + lane; x < np; x += WPR * 32) M = fmaxf(M, (x < own_n ? p.own_ml : p.pre_ml)[slot(x) * 2]);
   M = warp_max(M);
@@ -708,33 +763,41 @@ __global__ void __launch_bounds__(128) decode_combine_kernel(const AttnParams p)
   }
 }
 
-template <int H, bool Q8, int MT>
+template <int H, bool Q8, int MT, bool WHOLE>
 void launch_attn(const AttnParams& p) {
   constexpr int smem = Cfg<H, Q8, MT>::SMEM;
   static bool configured[64] = {};
   int dev = 0;
   HB_CUDA_CHECK(cudaGetDevice(&dev));
   if (!configured[dev & 63]) {
-    HB_CUDA_CHECK(cudaFuncSetAttribute(decode_attn_kernel<H, Q8, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    HB_CUDA_CHECK(cudaFuncSetAttribute(decode_attn_kernel<H, Q8, MT, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     configured[dev & 63] = true;
   }
-  const long long blocks = (long long)p.n_pre + (long long)p.n_suf * p.N * p.own_rt;
+  const long long blocks = WHOLE ? (long long)p.B * p.N * p.own_rt : p.n_pre + (long long)p.n_suf * p.N * p.own_rt;
   HB_CHECK(blocks < (1ll << 31), "decode_attention: too many tiles");
-  decode_attn_kernel<H, Q8, MT><<<(unsigned)blocks, WARPS * 32, smem, cur_stream()>>>(p);
-  HB_CUDA_CHECK(cudaGetLastError());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = cur_stream();
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = WHOLE && p.tc_ctas > 0 ? 1 : 0;   // starts while the prefix kernel ends
+  HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, decode_attn_kernel<H, Q8, MT, WHOLE>, p));
 }
 
 template <int H>
 void launch_combine(const AttnParams& p) {
   const long long rows = (long long)p.B * p.S * p.Nq;
   // few rows of many pieces: four warps a row
-  if (p.n_split + p.n_suf > 8 && rows <= 4096) decode_combine_kernel<H, 4><<<(unsigned)rows, 128, 0, cur_stream()>>>(p);
+  if (std::max(p.n_split, p.tc_ctas) + p.n_suf > 8 && rows <= 4096) decode_combine_kernel<H, 4><<<(unsigned)rows, 128, 0, cur_stream()>>>(p);
   else decode_combine_kernel<H, 1><<<(unsigned)((rows + 3) / 4), 128, 0, cur_stream()>>>(p);
   HB_CUDA_CHECK(cudaGetLastError());
 }
 
-KvView view_of(const torch::Tensor& k, const torch::Tensor& v, const c10::optional<torch::Tensor>& ke,
-               const c10::optional<torch::Tensor>& ve) {
+KvView view_of(const torch::Tensor& k, const torch::Tensor& v, const OptTensor& ke, const OptTensor& ve) {
   KvView o{};
   const long long es = k.element_size();
   o.k = (const uint8_t*)k.data_ptr(), o.v = (const uint8_t*)v.data_ptr();
@@ -751,24 +814,39 @@ KvView view_of(const torch::Tensor& k, const torch::Tensor& v, const c10::option
 }  // namespace
 
 // q [B, S, Nq, H] bf16, own caches [B, C, N, H], prefix caches [1, P, N, H] (or
-// none) -> out [B, S, Nq, H] bf16 contiguous.
-void decode_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::optional<torch::Tensor> k_exp,
-                      c10::optional<torch::Tensor> v_exp, c10::optional<torch::Tensor> pk,
-                      c10::optional<torch::Tensor> pv, c10::optional<torch::Tensor> pk_exp,
-                      c10::optional<torch::Tensor> pv_exp, torch::Tensor lengths, c10::optional<torch::Tensor> counts,
-                      int64_t window, double scale, torch::Tensor out) {
-  const c10::cuda::CUDAGuard guard(q.device());
-  const int H = (int)q.size(3);
-  HB_CHECK(H == 32 || H == 64 || H == 128, "decode_attention: head dim 32, 64 or 128");
+// none) -> [B, S, Nq, H] bf16 contiguous.
+torch::Tensor decode_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, OptTensor k_exp, OptTensor v_exp,
+                               OptTensor pk, OptTensor pv, OptTensor pk_exp, OptTensor pv_exp, torch::Tensor lengths,
+                               OptTensor counts, int64_t window, c10::optional<double> scale) {
+  const auto dev = q.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  need(q.dim() == 4 && q.scalar_type() == at::kBFloat16, "decode_attention: q [B, S, Nq, H], bf16");
+  check_cache(k, v, k_exp, v_exp, dev);
+  const int64_t B = q.size(0), S = q.size(1), Nq = q.size(2), H = q.size(3), N = k.size(2);
+  need(k.size(0) == B && k.size(3) == H && N > 0 && Nq % N == 0,
+       "decode_attention: a cache of q's B sequences and head dim, with KV heads that divide its heads");
+  if (pk) {
+    check_cache(*pk, *pv, pk_exp, pv_exp, dev);
+    need(pk->size(0) == 1 && pk->size(2) == N && pk->size(3) == H && pk->scalar_type() == k.scalar_type(),
+         "decode_attention: one prefix sequence [1, P, N, H] of the cache's type");
+  }
+  need(window >= 0, "decode_attention: window >= 0");
+  need(!scale || *scale > 0, "decode_attention: scale > 0");
+  need(!wants_grad(q) && !wants_grad(k) && !wants_grad(v), "decode_attention has no backward: call it under torch.no_grad()");
+  lengths = whole(lengths, B, dev, "decode_attention: lengths, B whole numbers on q's device");
+  if (counts) counts = whole(*counts, B, dev, "decode_attention: counts, B whole numbers on q's device");
+  torch::Tensor out = torch::empty({B, S, Nq, H}, q.options());
+  if (out.numel() == 0) return out;
+  q = aligned_rows(q);
   AttnParams p{};
-  p.B = (int)q.size(0), p.S = (int)q.size(1), p.Nq = (int)q.size(2), p.N = (int)k.size(2);
-  if (p.B == 0 || p.S == 0) return;
-  p.G = p.Nq / p.N, p.C = (int)k.size(1), p.P = pk ? (int)pk->size(1) : 0;
-  p.W = (int)window;
-  HB_CHECK((long long)p.P + p.C < (1ll << 30), "decode_attention: more than 2^30 keys");
-  HB_CHECK((long long)p.B * p.S * p.G < (1ll << 30), "decode_attention: more than 2^30 query rows");
+  p.B = (int)B, p.S = (int)S, p.Nq = (int)Nq, p.N = (int)N, p.G = (int)(Nq / N);
+  p.C = (int)k.size(1), p.P = pk ? (int)pk->size(1) : 0;
+  p.W = (int)std::min<int64_t>(window, 1ll << 30);
+  need((long long)p.P + k.size(1) < (1ll << 30), "decode_attention: at most 2^30 keys");
+  need(B * S * p.G < (1ll << 30), "decode_attention: at most 2^30 query rows");
   p.q = (const __nv_bfloat16*)q.data_ptr();
   p.qb = q.stride(0), p.qs = q.stride(1), p.qh = q.stride(2);
+  if (p.W == 1) p.P = 0;   // a query sees itself only
   const bool q8 = k_exp.has_value();
   p.own = view_of(k, v, k_exp, v_exp);
   if (p.P) {
@@ -777,42 +855,77 @@ void decode_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::op
   }
   p.lengths = lengths.data_ptr<int>();
   p.counts = counts ? counts->data_ptr<int>() : nullptr;
-  p.sl2 = (float)(scale * 1.4426950408889634);
+  p.sl2 = (float)((scale ? *scale : 1.0 / std::sqrt((double)H)) * 1.4426950408889634);
   p.out = (__nv_bfloat16*)out.data_ptr();
   p.status = status_ptr();
 
   const int SG = p.S * p.G, R = p.B * SG;
-  const int mt = SG > 16 || (p.P && R > 16) ? 2 : 1;
   const int sms = num_sms();
+  p.budget_ns = wait_budget_ns();
+  // Many rows that share the prefix: tcgen05 (128-row tiles); few: mma.sync.
+  const bool tc = p.P && H >= 64 && R > 64;
+  const int mt = SG > 16 || (p.P && !tc && R > 16) ? 2 : 1;
   p.own_rt = (SG + 16 * mt - 1) / (16 * mt);
+  // One CTA per (sequence, KV head) when those fill half the SMs and no sequence
+  // is long: it joins the prefix pieces itself (one launch less).  Not where
+  // the prefix runs on mma.sync, in the same launch as the own keys.
+  const bool whole = (!p.P || tc) && (long long)p.B * p.N * p.own_rt >= sms / 2 && p.C <= 2048;
   // own keys: about two CTAs per SM, at least 8 tiles of the full capacity each
   const long long cap_tiles = (long long)p.B * ((p.C + KB - 1) / KB);
   p.n_suf = (int)std::max<long long>(1, std::min<long long>(2ll * sms / ((long long)p.N * p.own_rt), cap_tiles / 8));
-  if (p.P) {
-    p.pre_lo = p.W > 0 ? std::max(0, p.P - p.W + 1) : 0;
+  long long pre_rows = 0;
+  if (p.P) p.pre_lo = p.W > 0 ? std::max(0, p.P - p.W + 1) : 0;
+  if (tc) {
+    p.tc_rows = R > 128 ? 256 : 128;
+    p.tc_rt = (R + p.tc_rows - 1) / p.tc_rows;
+    p.tc_tiles = (p.P - p.pre_lo + 127) / 128;
+    const long long units = (long long)p.N * p.tc_rt, total = units * p.tc_tiles;
+    p.tc_per = (int)((total + sms - 1) / sms);
+    p.tc_ctas = (int)((total + p.tc_per - 1) / p.tc_per);
+    pre_rows = (p.tc_ctas + units) * p.tc_rows;
+  } else if (p.P) {
     p.pre_rt = (R + 16 * mt - 1) / (16 * mt);
     const int tiles = (p.P - p.pre_lo + KB - 1) / KB;
     p.n_split = (int)std::max<long long>(1, std::min<long long>(2ll * sms / ((long long)p.N * p.pre_rt), tiles / 8));
     p.n_pre = p.n_split * p.N * p.pre_rt;
+    pre_rows = (long long)p.N * p.n_split * R;
   }
   // workspace: own slots, prefix slots, tile starts
-  const long long own_rows = (long long)p.N * (p.n_suf + p.B) * SG, pre_rows = (long long)p.N * p.n_split * R;
+  const long long own_rows = whole ? 0 : (long long)p.N * (p.n_suf + p.B) * SG;
   torch::Tensor ws = torch::empty({(own_rows + pre_rows) * (H + 2) + p.B + 1}, q.options().dtype(torch::kFloat));
   p.own_o = ws.data_ptr<float>();
   p.pre_o = p.own_o + own_rows * H;
   p.own_ml = p.pre_o + pre_rows * H;
   p.pre_ml = p.own_ml + own_rows * 2;
   p.tile_start = reinterpret_cast<int*>(p.pre_ml + pre_rows * 2);
-#define HB_ATTN(HH)                                                               \
-  do {                                                                            \
-    if (q8) mt == 2 ? launch_attn<HH, true, 2>(p) : launch_attn<HH, true, 1>(p);  \
-    else mt == 2 ? launch_attn<HH, false, 2>(p) : launch_attn<HH, false, 1>(p);   \
-    launch_combine<HH>(p);                                                        \
+  if (tc) {
+    if (q8) {   // the prefix's values, once for all rows
+      auto [k16, v16] = kv_cache_read(*pk, *pv, pk_exp, pv_exp, c10::nullopt, p.P);
+      prefix_tc_launch(p, (int)H, k16.data_ptr(), v16.data_ptr(), N * H * 2, H * 2, N * H * 2, H * 2);
+    } else {
+      prefix_tc_launch(p, (int)H, p.pre.k, p.pre.v, p.pre.ks, p.pre.kn, p.pre.vs, p.pre.vn);
+    }
+  }
+#define HB_ATTN2(HH, W)                                                                 \
+  do {                                                                                  \
+    if (q8) mt == 2 ? launch_attn<HH, true, 2, W>(p) : launch_attn<HH, true, 1, W>(p);  \
+    else mt == 2 ? launch_attn<HH, false, 2, W>(p) : launch_attn<HH, false, 1, W>(p);   \
+  } while (0)
+#define HB_ATTN(HH)          \
+  do {                       \
+    if (whole) {             \
+      HB_ATTN2(HH, true);    \
+    } else {                 \
+      HB_ATTN2(HH, false);   \
+      launch_combine<HH>(p); \
+    }                        \
   } while (0)
   if (H == 32) HB_ATTN(32);
   else if (H == 64) HB_ATTN(64);
   else HB_ATTN(128);
 #undef HB_ATTN
+#undef HB_ATTN2
+  return out;
 }
 
 }  // namespace hb

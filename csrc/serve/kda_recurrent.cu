@@ -14,6 +14,7 @@
 
 #include "../common/host.h"
 #include "../common/sm100.cuh"
+#include "checks.h"
 
 namespace hb {
 namespace {
@@ -236,16 +237,43 @@ Row3 row3(const torch::Tensor& t) { return {t.stride(0), t.stride(1), t.stride(2
 
 }  // namespace
 
-// q, k, v [B, S, H, K] (fp32 or bf16, rows contiguous), g like them in fp32,
-// beta [B, S, H] fp32, s0 [B or 1, H, K, K] fp32 or none -> o [B, S, H, K] and
-// s1 [B, H, K, K], both fp32 and contiguous.
-void kda_recurrent(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor g, torch::Tensor beta, double scale,
-                   c10::optional<torch::Tensor> s0, c10::optional<torch::Tensor> counts, torch::Tensor o,
-                   torch::Tensor s1) {
-  const c10::cuda::CUDAGuard guard(q.device());
+// q, k, v [B, S, H, K] (fp32 or bf16), g like them in fp32, beta [B, S, H] fp32,
+// s0 [B or 1, H, K, K] fp32 or none -> o [B, S, H, K] and s1 [B, H, K, K], both
+// fp32 and contiguous.
+std::tuple<torch::Tensor, torch::Tensor> kda_recurrent(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor g,
+                                                       torch::Tensor beta, c10::optional<double> scale, OptTensor s0,
+                                                       OptTensor counts) {
+  const auto dev = q.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  need(q.dim() == 4 && k.sizes() == q.sizes() && v.sizes() == q.sizes() && g.sizes() == q.sizes() &&
+           beta.sizes() == q.sizes().slice(0, 3),
+       "kda_recurrent: q, k, v, g [B, S, H, K] and beta [B, S, H]");
+  need(k.device() == dev && v.device() == dev && g.device() == dev && beta.device() == dev,
+       "kda_recurrent: all inputs on one device");
+  need(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type() &&
+           (q.scalar_type() == at::kFloat || q.scalar_type() == at::kBFloat16) && g.scalar_type() == at::kFloat &&
+           beta.scalar_type() == at::kFloat,
+       "kda_recurrent: fp32 or bf16 q, k, v; fp32 g and beta");
   const int64_t B = q.size(0), S = q.size(1), H = q.size(2), K = q.size(3);
-  HB_CHECK(K == 16 || K == 32 || K == 64 || K == 128, "kda_recurrent: head dim 16, 32, 64 or 128");
-  if (B * H == 0) return;
+  need(K == 16 || K == 32 || K == 64 || K == 128, "kda_recurrent: head dim 16, 32, 64 or 128");
+  if (s0)
+    need(s0->dim() == 4 && (s0->size(0) == 1 || s0->size(0) == B) && s0->size(1) == H && s0->size(2) == K &&
+             s0->size(3) == K && s0->device() == dev && s0->scalar_type() == at::kFloat,
+         "kda_recurrent: state [B or 1, H, K, K] fp32 on the inputs' device");
+  for (const auto& t : {q, k, v, g, beta}) need(!wants_grad(t), "kda_recurrent has no backward: call it under torch.no_grad()");
+  need(!s0 || !wants_grad(*s0), "kda_recurrent has no backward: call it under torch.no_grad()");
+  if (counts) counts = whole(*counts, B, dev, "kda_recurrent: counts, B whole numbers on the inputs' device");
+  const auto opt = q.options().dtype(at::kFloat);
+  torch::Tensor o = torch::empty({B, S, H, K}, opt), s1 = torch::empty({B, H, K, K}, opt);
+  if (B * H == 0) return {o, s1};
+  const auto rows = [](const torch::Tensor& t) { return t.stride(3) == 1 ? t : t.contiguous(); };
+  q = rows(q), k = rows(k), v = rows(v), g = rows(g);
+  if (s0) {   // 16-byte loads of contiguous states; a broadcast over the batch stays one
+    const auto z = s0->stride(0) == 0 && B > 1 ? s0->narrow(0, 0, 1) : *s0;
+    const bool ok = z.select(0, 0).is_contiguous() && reinterpret_cast<uintptr_t>(z.data_ptr()) % 16 == 0 &&
+                    (z.size(0) == 1 || z.stride(0) % 4 == 0);
+    s0 = ok ? z : z.clone(at::MemoryFormat::Contiguous);
+  }
   RecParams p{};
   p.q = q.data_ptr(), p.k = k.data_ptr(), p.v = v.data_ptr();
   p.g = g.data_ptr<float>(), p.beta = beta.data_ptr<float>();
@@ -255,10 +283,11 @@ void kda_recurrent(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Ten
   p.s1 = s1.data_ptr<float>(), p.o = o.data_ptr<float>();
   p.counts = counts ? counts->data_ptr<int>() : nullptr;
   p.B = (int)B, p.S = (int)S, p.H = (int)H;
-  p.scale = (float)scale;
+  p.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)K));
   p.status = status_ptr();
   if (q.scalar_type() == at::kFloat) dispatch_rec<float>(p, (int)K);
   else dispatch_rec<__nv_bfloat16>(p, (int)K);
+  return {o, s1};
 }
 
 }  // namespace hb

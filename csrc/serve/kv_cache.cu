@@ -17,6 +17,7 @@
 
 #include "../common/host.h"
 #include "../common/sm100.cuh"
+#include "checks.h"
 
 namespace hb {
 namespace {
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p) {
   const int l = threadIdx.x % LPR;
   const unsigned n = row % p.N, bs = row / p.N, i = bs % p.S, b = bs / p.S;
   if (b >= p.B) return;
-  const long long at = (long long)p.starts[b] + i;
+  const long long at = (p.starts ? (long long)p.starts[b] : 0) + i;
   uint4 o = make_uint4(0, 0, 0, 0);
   if (index_ok(at, p.C, p.status)) {
     const long long off = b * sd.cs.b + at * sd.cs.s + n * sd.cs.n + l * 8;
@@ -165,14 +166,6 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p) {
 
 RowStrides strides_of(const torch::Tensor& t) { return {t.stride(0), t.stride(1), t.stride(2)}; }
 
-void check_rows(const torch::Tensor& t, const char* name) {
-  HB_CHECK(t.is_cuda() && t.dim() == 4 && t.stride(3) == 1, std::string(name) + ": CUDA [B, S, N, H] with contiguous rows");
-  const int64_t es = t.element_size();
-  HB_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, std::string(name) + ": 16-byte aligned");
-  for (int i = 0; i < 3; ++i)
-    HB_CHECK(t.size(i) <= 1 || t.stride(i) * es % 16 == 0, std::string(name) + ": strides of whole 16-byte units");
-}
-
 template <typename T, bool QUANT>
 void launch_write(const WriteParams& p, int H, dim3 grid) {
   if (H == 32) kv_write_kernel<T, 32, QUANT><<<grid, 256, 0, cur_stream()>>>(p);
@@ -189,18 +182,23 @@ dim3 rows_grid(int64_t rows, int64_t H) {
 }  // namespace
 
 // k, v [B, S, N, H] bf16 or fp32 into rows starts[b] + i (i < counts[b]) of the
-// caches [B, C, N, H] (e4m3 with int8 exponents [B, C, N], or bf16).
-void kv_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, torch::Tensor v_cache,
-                    c10::optional<torch::Tensor> k_exp, c10::optional<torch::Tensor> v_exp, torch::Tensor starts,
-                    c10::optional<torch::Tensor> counts) {
-  const c10::cuda::CUDAGuard guard(k.device());
-  check_rows(k, "kv_cache_write: k");
-  check_rows(v, "kv_cache_write: v");
-  check_rows(k_cache, "kv_cache_write: k cache");
-  check_rows(v_cache, "kv_cache_write: v cache");
-  const int64_t B = k.size(0), S = k.size(1), N = k.size(2), H = k.size(3);
+// caches [B, C, N, H].
+void kv_cache_write(torch::Tensor k_cache, torch::Tensor v_cache, OptTensor k_exp, OptTensor v_exp, torch::Tensor k,
+                    torch::Tensor v, torch::Tensor starts, OptTensor counts) {
+  const auto dev = k_cache.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  check_cache(k_cache, v_cache, k_exp, v_exp, dev);
+  const int64_t B = k_cache.size(0), N = k_cache.size(2), H = k_cache.size(3);
+  need(k.dim() == 4 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.device() == dev &&
+           v.device() == dev && k.size(0) == B && k.size(2) == N && k.size(3) == H,
+       "kv_cache_write: keys and values [B, S, N, H] of one type, shaped like the cache and on its device");
+  need(k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kFloat, "kv_cache_write: bf16 or fp32 rows");
+  need(!wants_grad(k) && !wants_grad(v), "kv_cache_write has no backward: call it under torch.no_grad()");
+  const int64_t S = k.size(1);
+  starts = whole(starts, B, dev, "kv_cache_write: starts, B whole numbers on the cache's device");
+  if (counts) counts = whole(*counts, B, dev, "kv_cache_write: counts, B whole numbers on the cache's device");
   if (B * S * N == 0) return;
-  HB_CHECK(H == 32 || H == 64 || H == 128, "kv_cache_write: head dim 32, 64 or 128");
+  k = aligned_rows(k), v = aligned_rows(v);
   const bool quant = k_exp.has_value();
   WriteParams p{};
   p.side[0] = {k.data_ptr(), k_cache.data_ptr(), quant ? k_exp->data_ptr<int8_t>() : nullptr, strides_of(k),
@@ -216,30 +214,31 @@ void kv_cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor k_cache, tor
     if (quant) launch_write<__nv_bfloat16, true>(p, (int)H, grid);
     else launch_write<__nv_bfloat16, false>(p, (int)H, grid);
   } else {
-    HB_CHECK(k.scalar_type() == at::kFloat, "kv_cache_write: bf16 or fp32 rows");
     if (quant) launch_write<float, true>(p, (int)H, grid);
     else launch_write<float, false>(p, (int)H, grid);
   }
   HB_CUDA_CHECK(cudaGetLastError());
 }
 
-// Rows starts[b] .. starts[b] + S - 1 of the caches as bf16 [B, S, N, H].
-void kv_cache_read(torch::Tensor k_cache, torch::Tensor v_cache, c10::optional<torch::Tensor> k_exp,
-                   c10::optional<torch::Tensor> v_exp, torch::Tensor starts, torch::Tensor k_out,
-                   torch::Tensor v_out) {
-  const c10::cuda::CUDAGuard guard(k_cache.device());
-  check_rows(k_cache, "kv_cache_read: k cache");
-  check_rows(v_cache, "kv_cache_read: v cache");
-  const int64_t B = k_out.size(0), S = k_out.size(1), N = k_out.size(2), H = k_out.size(3);
-  if (B * S * N == 0) return;
-  HB_CHECK(H == 32 || H == 64 || H == 128, "kv_cache_read: head dim 32, 64 or 128");
+// Rows starts[b] .. starts[b] + S - 1 (from 0 without starts) of the caches as bf16 [B, S, N, H].
+std::tuple<torch::Tensor, torch::Tensor> kv_cache_read(torch::Tensor k_cache, torch::Tensor v_cache, OptTensor k_exp,
+                                                       OptTensor v_exp, OptTensor starts, int64_t S) {
+  const auto dev = k_cache.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  check_cache(k_cache, v_cache, k_exp, v_exp, dev);
+  const int64_t B = k_cache.size(0), N = k_cache.size(2), H = k_cache.size(3);
+  need(S >= 0, "kv_cache_read: n >= 0");
+  if (starts) starts = whole(*starts, B, dev, "kv_cache_read: starts, B whole numbers on the cache's device");
+  const auto opt = k_cache.options().dtype(at::kBFloat16);
+  torch::Tensor k_out = torch::empty({B, S, N, H}, opt), v_out = torch::empty({B, S, N, H}, opt);
+  if (B * S * N == 0) return {k_out, v_out};
   const bool quant = k_exp.has_value();
   ReadParams p{};
   p.side[0] = {k_cache.data_ptr(), quant ? k_exp->data_ptr<int8_t>() : nullptr, (__nv_bfloat16*)k_out.data_ptr(),
                strides_of(k_cache), quant ? strides_of(*k_exp) : RowStrides{}};
   p.side[1] = {v_cache.data_ptr(), quant ? v_exp->data_ptr<int8_t>() : nullptr, (__nv_bfloat16*)v_out.data_ptr(),
                strides_of(v_cache), quant ? strides_of(*v_exp) : RowStrides{}};
-  p.starts = starts.data_ptr<int>();
+  p.starts = starts ? starts->data_ptr<int>() : nullptr;
   p.B = (unsigned)B, p.S = (unsigned)S, p.N = (unsigned)N, p.C = (int)k_cache.size(1);
   p.status = status_ptr();
   const dim3 grid = rows_grid(B * S * N, H);
@@ -254,6 +253,7 @@ void kv_cache_read(torch::Tensor k_cache, torch::Tensor v_cache, c10::optional<t
     else kv_read_kernel<128, false><<<grid, 256, 0, st>>>(p);
   }
   HB_CUDA_CHECK(cudaGetLastError());
+  return {k_out, v_out};
 }
 
 }  // namespace hb

@@ -1,0 +1,370 @@
+// Prefix part of the decoding attention on tcgen05: the rows of all sequences of
+// a batch (B * S * G per KV head) against the keys that they share.
+//
+// A unit is (KV head, NS * 128 rows); its keys come in tiles of 128.  The tiles
+// of all units are laid end to end and cut into equal ranges, one per CTA (one
+// CTA per SM); piece (CTA c, unit u) leaves (O, m, l) of its rows in slot c + u,
+// since along the tiles each new piece starts a new CTA or a new unit.
+//
+// Warps: 4 NS softmax warps (one thread per row), a TMA producer and an MMA
+// issuer.  Each 128-row stream has its score tile S [128 x 128] and output O
+// [128 x H] in TMEM:
+//   S_j = Q K_j^T            operands in shared memory
+//   P_j = 2^{S_j sl2 - m}    a thread reads its whole row of S into registers,
+//                            and writes P as bf16 pairs back to TMEM
+//   O  += P_j V_j            A operand from TMEM
+// Head dim 64: P has columns of its own, so S_{j+1} is computed while the softmax
+// of S_j runs.  Head dim 128: the TMEM (512 columns) is full, P overlays S, and
+// S_{j+1} follows P_j V_j; the two streams alternate on the tensor cores.
+// The maximum used is raised only when a tile exceeds it by more than 2^8, so O
+// is rescaled rarely and P stays <= 256.
+#include <torch/extension.h>
+
+#include "../common/host.h"
+#include "attn_params.cuh"
+
+namespace hb {
+namespace {
+
+constexpr int TK = 128;   // keys per tile
+
+template <int H, int NS>
+struct Tc {
+  static constexpr int Q_BYTES = 128 * H * 2;   // per stream
+  static constexpr int T_BYTES = TK * H * 2;    // K or V tile
+  static constexpr int ST = H == 64 ? 3 : 2;    // stages of K and of V
+  static constexpr int THREADS = NS == 2 ? 384 : 192;
+  static constexpr bool OVERLAY = H == 128;
+  // TMEM columns
+  static constexpr int S_COL(int st) { return OVERLAY ? st * 128 : st * 192; }
+  static constexpr int P_COL(int st) { return OVERLAY ? st * 128 : st * 192 + 128; }
+  static constexpr int O_COL(int st) { return OVERLAY ? 256 + st * 128 : 384 + st * 64; }
+  static constexpr int SMEM = 1024 + NS * Q_BYTES + 2 * ST * T_BYTES + 512;
+};
+
+HB_DEVICE uint64_t k_desc(uint32_t base, int kk) {   // K step kk (16) of a 128-row K-major tile
+  return make_smem_desc(base + (kk >> 2) * 128 * 128 + (kk & 3) * 32, 16, 1024);
+}
+// D += A B with A in TMEM
+HB_DEVICE void umma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+// 32 lanes x 16 consecutive 32-bit columns <- 16 registers per thread.
+HB_DEVICE void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+template <int H, int NS>
+__global__ void __launch_bounds__(Tc<H, NS>::THREADS, 1)
+    prefix_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const AttnParams p) {
+  using F = Tc<H, NS>;
+  constexpr int ST = F::ST;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sQ = smem_u32(smem), sK = sQ + NS * F::Q_BYTES, sV = sK + ST * F::T_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + NS * F::Q_BYTES + 2 * ST * F::T_BYTES);
+  uint64_t *k_full = bars, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
+  uint64_t *q_full = v_empty + ST, *s_full = q_full + NS, *s_read = s_full + NS, *p_full = s_read + NS, *pv_done = p_full + NS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + NS);
+
+  launch_dependents();
+  const int warp = threadIdx.x / 32;
+  const int R = p.B * p.S * p.G, SG = p.S * p.G;
+  const long long total = (long long)p.N * p.tc_rt * p.tc_tiles;
+  const long long t_begin = (long long)blockIdx.x * p.tc_per;
+  const int n_it = (int)(min(total, t_begin + p.tc_per) - t_begin);   // tiles of this CTA
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(smem_u32(&k_full[i]), 1), mbar_init(smem_u32(&k_empty[i]), 1);
+      mbar_init(smem_u32(&v_full[i]), 1), mbar_init(smem_u32(&v_empty[i]), 1);
+    }
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(smem_u32(&q_full[i]), 128), mbar_init(smem_u32(&s_full[i]), 1), mbar_init(smem_u32(&s_read[i]), 128);
+      mbar_init(smem_u32(&p_full[i]), 128), mbar_init(smem_u32(&pv_done[i]), 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == NS * 4 + 1) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // Two streams: 384 threads start with 168 registers; a softmax thread holds its
+  // row of 128 scores and takes 208 (256 x 208 + 128 x 88 = 384 x 168).
+  if (warp >= NS * 4) {
+    if constexpr (NS == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp == NS * 4) {
+    // ------------------------------------------------------------ producer
+    if (elect_one()) {
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+      for (int it = 0; it < n_it; ++it) {
+        const int st = it % ST, par = ((it / ST) & 1) ^ 1;
+        const long long tile = t_begin + it;
+        const int n = (int)(tile / p.tc_tiles / p.tc_rt), key = p.pre_lo + (int)(tile % p.tc_tiles) * TK;
+        if (!mbar_wait(smem_u32(&k_empty[st]), par, p.status, kErrTimeoutProducer, p.budget_ns)) break;
+        mbar_expect_tx(smem_u32(&k_full[st]), F::T_BYTES);
+        for (int a = 0; a < H / 64; ++a)
+          tma_load_3d(sK + st * F::T_BYTES + a * TK * 128, &tmK, smem_u32(&k_full[st]), 64 * a, key, n);
+        if (!mbar_wait(smem_u32(&v_empty[st]), par, p.status, kErrTimeoutProducer, p.budget_ns)) break;
+        mbar_expect_tx(smem_u32(&v_full[st]), F::T_BYTES);
+        for (int a = 0; a < H / 64; ++a)
+          tma_load_3d(sV + st * F::T_BYTES + a * TK * 128, &tmV, smem_u32(&v_full[st]), 64 * a, key, n);
+      }
+    }
+  } else if (warp == NS * 4 + 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (elect_one()) {
+      constexpr uint32_t id_s = make_idesc_bf16(128, TK, false, false);
+      constexpr uint32_t id_o = make_idesc_bf16(128, H, false, true);
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int parity) {
+        if (ok) ok = mbar_wait(smem_u32(bar), parity, p.status, kErrTimeoutMma, p.budget_ns);
+        return ok;
+      };
+      auto issue_s = [&](int st, int it) {
+        const uint32_t k = sK + it % ST * F::T_BYTES, q = sQ + st * F::Q_BYTES;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < H / 16; ++kk)
+          umma_f16(tmem + F::S_COL(st), k_desc(q, kk), k_desc(k, kk), id_s, kk != 0 ? 1u : 0u);
+        umma_commit(smem_u32(&s_full[st]));
+      };
+      auto issue_pv = [&](int st, int it, bool first) {
+        const uint32_t v = sV + it % ST * F::T_BYTES;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < TK / 16; ++kk)
+          umma_f16_ta(tmem + F::O_COL(st), tmem + F::P_COL(st) + kk * 8, make_smem_desc(v + kk * 2048, TK * 128, 1024), id_o,
+                      first && kk == 0 ? 0u : 1u);
+        umma_commit(smem_u32(&pv_done[st]));
+      };
+      int piece = 0;
+      auto first_s = [&](int it) {   // scores of a piece's first tile
+        for (int st = 0; st < NS; ++st) {
+          if (!wait(&q_full[st], piece & 1)) return;
+          if (st == 0 && !wait(&k_full[it % ST], (it / ST) & 1)) return;
+          issue_s(st, it);
+        }
+        umma_commit(smem_u32(&k_empty[it % ST]));
+      };
+      first_s(0);
+      for (int it = 0; ok && it < n_it; ++it) {
+        const long long tile = t_begin + it;
+        const bool first = it == 0 || tile % p.tc_tiles == 0, last = (tile + 1) % p.tc_tiles == 0;
+        const bool more = it + 1 < n_it && !last;   // the next tile is of the same piece
+        if constexpr (!F::OVERLAY) {
+          if (more) {
+            for (int st = 0; st < NS; ++st) {
+              if (st == 0 && !wait(&k_full[(it + 1) % ST], ((it + 1) / ST) & 1)) break;
+              if (!wait(&s_read[st], it & 1)) break;
+              issue_s(st, it + 1);
+            }
+            if (ok) umma_commit(smem_u32(&k_empty[(it + 1) % ST]));
+          }
+        }
+        for (int st = 0; ok && st < NS; ++st) {
+          if (st == 0 && !wait(&v_full[it % ST], (it / ST) & 1)) break;
+          if (!wait(&p_full[st], it & 1)) break;
+          issue_pv(st, it, first);
+          if constexpr (F::OVERLAY) {
+            if (more) {   // P overlays S: the product that reads P has to end first
+              if (st == 0 && !wait(&k_full[(it + 1) % ST], ((it + 1) / ST) & 1)) break;
+              if (!wait(&pv_done[st], it & 1)) break;
+              issue_s(st, it + 1);
+            }
+          }
+        }
+        if (!ok) break;
+        umma_commit(smem_u32(&v_empty[it % ST]));
+        if constexpr (F::OVERLAY) {
+          if (more) umma_commit(smem_u32(&k_empty[(it + 1) % ST]));
+        }
+        if (it + 1 < n_it && last) {
+          ++piece;
+          first_s(it + 1);
+        }
+      }
+    }
+  }
+  } else {
+    // ------------------------------------------------------------ softmax: one thread per row
+    if constexpr (NS == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int st = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tS = lanes + F::S_COL(st), tP = lanes + F::P_COL(st), tO = lanes + F::O_COL(st);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, int parity) {
+      if (ok) ok = mbar_wait(smem_u32(bar), parity, p.status, kErrTimeoutEpilogue, p.budget_ns);
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    int it = 0;
+    while (it < n_it) {   // pieces
+      const long long tile = t_begin + it;
+      const int u = (int)(tile / p.tc_tiles), n = u / p.tc_rt, rt = u % p.tc_rt;
+      int kt = (int)(tile % p.tc_tiles);
+      const int tiles = min(n_it - it, p.tc_tiles - kt);
+      const int rr = rt * (NS * 128) + st * 128 + r;
+      const bool real = rr < R;
+      int lo = 0;
+      {   // this thread's row of Q into the swizzled K-major tile
+        const int b = real ? rr / SG : 0, ri = real ? rr % SG : 0, i = ri / p.G;
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + b * p.qb + i * p.qs + (long long)(n * p.G + ri % p.G) * p.qh);
+        const uint32_t row = sQ + st * F::Q_BYTES + r * 128;
+#pragma unroll
+        for (int c = 0; c < H / 8; ++c) {
+          const uint4 x = real ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (c >> 3) * 128 * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                       "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
+                       : "memory");
+        }
+        if (p.W > 0 && real) {
+          const int len = len_of(p, b, false), cnt = count_of(p, b, len, false);
+          if (i < cnt) lo = max(0, p.P + len - cnt + i - p.W + 1);
+        }
+      }
+      fence_proxy_async();
+      mbar_arrive(smem_u32(&q_full[st]));
+
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < tiles; ++j, ++it, ++kt) {
+        wait(&s_full[st], it & 1);
+        tc_fence_after();
+        const int key0 = p.pre_lo + kt * TK;
+        const bool edge = key0 + TK > p.P || (p.W > 0 && key0 < lo);
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(tS + 32 * c, s[c]);
+        tmem_ld_wait();
+        if constexpr (!F::OVERLAY) {
+          tc_fence_before();
+          mbar_arrive(smem_u32(&s_read[st]));
+        }
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (key0 + 32 * c + e >= p.P || key0 + 32 * c + e < lo) s[c][e] = __float_as_uint(-INFINITY);
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.sl2;
+        const bool raise = mt > m + 8.f;
+        float alpha = 1.f;
+        if (raise) {
+          alpha = m == -INFINITY ? 0.f : ex2f(m - mt);
+          m = mt;
+          l *= alpha;
+        }
+        const bool warp_raise = __any_sync(0xffffffffu, raise);
+        if (j > 0) {   // O and P are free once the previous product has ended
+          wait(&pv_done[st], (it - 1) & 1);
+          if (warp_raise) {
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < H / 32; ++c) {
+              uint32_t v[32];
+              tmem_ld_32x32b_x32(tO + 32 * c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+              tmem_st_32x32b_x32(tO + 32 * c, v);
+            }
+          }
+        }
+        const float nm = m == -INFINITY ? 0.f : -m;
+        const uint64_t sl2_2 = pack2(p.sl2, p.sl2), nm_2 = pack2(nm, nm);
+        uint64_t ls[2] = {0, 0};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float x0, x1;
+            unpack2(fma2(pack2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), sl2_2, nm_2), x0, x1);
+            x0 = ex2f(x0), x1 = ex2f(x1);
+            ls[e / 2 & 1] = add2(ls[e / 2 & 1], pack2(x0, x1));
+            w[e / 2] = pack_bf16x2(x0, x1);
+          }
+          tmem_st_x16(tP + 16 * c, w);
+        }
+        float l0, l1;
+        unpack2(add2(ls[0], ls[1]), l0, l1);
+        l += l0 + l1;
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&p_full[st]));
+      }
+      wait(&pv_done[st], (it - 1) & 1);
+      tc_fence_after();
+      const long long at = ((long long)blockIdx.x + u) * (NS * 128) + st * 128 + r;
+#pragma unroll
+      for (int c = 0; c < H / 32; ++c) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tO + 32 * c, v);
+        tmem_ld_wait();
+        if (real && ok) {
+          float4* o = reinterpret_cast<float4*>(p.pre_o + at * H + 32 * c);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            o[e] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]), __uint_as_float(v[4 * e + 2]),
+                               __uint_as_float(v[4 * e + 3]));
+        }
+      }
+      if (real) *reinterpret_cast<float2*>(p.pre_ml + at * 2) = make_float2(m, l);
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == NS * 4 + 1) tmem_dealloc(tmem, 512);
+}
+
+template <int H, int NS>
+void launch(const AttnParams& p, const CUtensorMap& tk, const CUtensorMap& tv) {
+  static bool configured[64] = {};
+  int dev = 0;
+  HB_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!configured[dev & 63]) {
+    HB_CUDA_CHECK(cudaFuncSetAttribute(prefix_tc_kernel<H, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tc<H, NS>::SMEM));
+    configured[dev & 63] = true;
+  }
+  prefix_tc_kernel<H, NS><<<p.tc_ctas, Tc<H, NS>::THREADS, Tc<H, NS>::SMEM, cur_stream()>>>(tk, tv, p);
+  HB_CUDA_CHECK(cudaGetLastError());
+}
+
+}  // namespace
+
+void prefix_tc_launch(const AttnParams& p, int H, const void* k, const void* v, long long ks, long long kn, long long vs,
+                      long long vn) {
+  const auto map = [&](const void* base, long long row, long long head) {
+    const uint64_t dims[3] = {(uint64_t)H, (uint64_t)p.P, (uint64_t)p.N};
+    // a stride over one head is never taken, but has to be valid
+    const uint64_t strides[2] = {(uint64_t)row, (uint64_t)(p.N > 1 ? head : row)};
+    const uint32_t box[3] = {64, TK, 1};
+    return make_tmap(base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  const CUtensorMap tk = map(k, ks, kn), tv = map(v, vs, vn);
+  if (H == 64) p.tc_rows == 256 ? launch<64, 2>(p, tk, tv) : launch<64, 1>(p, tk, tv);
+  else p.tc_rows == 256 ? launch<128, 2>(p, tk, tv) : launch<128, 1>(p, tk, tv);
+}
+
+}  // namespace hb

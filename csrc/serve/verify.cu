@@ -23,6 +23,7 @@
 
 #include "../common/host.h"
 #include "../common/sm100.cuh"
+#include "checks.h"
 
 namespace hb {
 namespace {
@@ -357,14 +358,45 @@ void launch_verify(const VerifyParams& p) {
 
 }  // namespace
 
-void verify_draft(torch::Tensor target, c10::optional<torch::Tensor> draft, torch::Tensor tokens, torch::Tensor uniform,
-                  torch::Tensor noise, c10::optional<torch::Tensor> lens, c10::optional<torch::Tensor> temperature,
-                  double temp, torch::Tensor out, torch::Tensor accepted, torch::Tensor logp) {
-  const c10::cuda::CUDAGuard guard(target.device());
+// target [B, K + 1, V], draft [B, K, V] or none -> tokens [B, K + 1], accepted
+// [B], log probabilities [B, K + 1].
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> verify_draft(torch::Tensor target, torch::Tensor tokens,
+                                                                     torch::Tensor uniform, torch::Tensor noise,
+                                                                     OptTensor draft, OptTensor lens,
+                                                                     OptTensor temperature, double temp) {
+  const auto dev = target.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  need(target.dim() == 3 && target.size(1) >= 1 && target.size(2) >= 1, "verify_draft: target logits [B, K + 1, V]");
+  need(target.scalar_type() == at::kFloat || target.scalar_type() == at::kBFloat16, "verify_draft: fp32 or bf16 logits");
+  const int64_t B = target.size(0), K = target.size(1) - 1, V = target.size(2);
+  need(K <= 32, "verify_draft: at most 32 drafted tokens");
+  need(V < (1ll << 30), "verify_draft: at most 2^30 logits a row");
+  const auto is = [&](const torch::Tensor& t, int64_t n, at::ScalarType ty) {
+    return t.dim() == 2 && t.size(0) == B && t.size(1) == n && t.scalar_type() == ty && t.device() == dev;
+  };
+  need(is(tokens, K, at::kLong), "verify_draft: drafted tokens [B, K] int64");
+  need(is(uniform, K, at::kFloat), "verify_draft: uniform [B, K] fp32");
+  need(is(noise, V, at::kFloat), "verify_draft: noise [B, V] fp32");
+  if (draft)
+    need(draft->dim() == 3 && draft->size(0) == B && draft->size(1) == K && draft->size(2) == V &&
+             draft->scalar_type() == target.scalar_type() && draft->device() == dev,
+         "verify_draft: draft logits [B, K, V] of the target's type");
+  if (lens) lens = whole(*lens, B, dev, "verify_draft: draft_lens, B whole numbers on the logits' device");
+  if (temperature) {
+    need(temperature->dim() == 1 && temperature->size(0) == B && temperature->scalar_type() == at::kFloat &&
+             temperature->device() == dev,
+         "verify_draft: temperature [B] fp32, or a number");
+    temperature = temperature->contiguous();
+  }
+  need(!wants_grad(target) && !(draft && wants_grad(*draft)), "verify_draft has no backward: call it under torch.no_grad()");
+  const auto opt = target.options();
+  torch::Tensor out = torch::empty({B, K + 1}, opt.dtype(at::kLong)), accepted = torch::empty({B}, opt.dtype(at::kLong)),
+                logp = torch::empty({B, K + 1}, opt.dtype(at::kFloat));
+  if (B == 0) return {out, accepted, logp};
+  target = target.contiguous(), tokens = tokens.contiguous(), uniform = uniform.contiguous(), noise = noise.contiguous();
+  if (draft) draft = draft->contiguous();
   VerifyParams p{};
-  p.B = (int)target.size(0), p.K = (int)target.size(1) - 1, p.V = (int)target.size(2);
-  HB_CHECK(p.K >= 0 && p.K <= 32, "verify_draft: 0 to 32 drafted tokens");
-  if (p.B == 0) return;
+  p.B = (int)B, p.K = (int)K, p.V = (int)V;
   p.target = target.data_ptr();
   p.draft = draft ? draft->data_ptr() : nullptr;
   p.tokens = (const long long*)tokens.data_ptr<int64_t>();
@@ -377,6 +409,7 @@ void verify_draft(torch::Tensor target, c10::optional<torch::Tensor> draft, torc
   p.status = status_ptr();
   if (target.scalar_type() == at::kFloat) launch_verify<float>(p);
   else launch_verify<__nv_bfloat16>(p);
+  return {out, accepted, logp};
 }
 
 }  // namespace hb

@@ -20,6 +20,8 @@ import torch
 from . import reference as ref
 from ._ext import available as ext_available  # noqa: F401
 from ._ext import check_status, ext  # noqa: F401
+from . import kv_cache as _kv
+from . import spec as _spec
 from .kv_cache import KVCache, new_kv_cache  # noqa: F401
 
 
@@ -88,15 +90,13 @@ def kv_cache_write(cache: KVCache, k, v, starts, counts=None) -> None:
     infinities saturated, NaN kept.  ``starts`` / ``counts``: whole numbers [B]
     on the device, or one int for all.  On the GPU a row outside the cache is
     skipped and recorded in the status word."""
-    from .kv_cache import kv_cache_write as f
-    f(cache, k, v, starts, counts)
+    _kv.kv_cache_write(cache, k, v, starts, counts)
 
 
 def kv_cache_read(cache: KVCache, starts, n: int):
     """Rows ``starts[b] .. starts[b] + n - 1`` of every sequence as values
     ``(k, v) [B, n, Nkv, H]`` (bf16 on the GPU, exact for either cache type)."""
-    from .kv_cache import kv_cache_read as f
-    return f(cache, starts, n)
+    return _kv.kv_cache_read(cache, starts, n)
 
 
 def decode_attention(q, cache: KVCache, lengths, counts=None, prefix: Optional[KVCache] = None, window: int = 0,
@@ -110,8 +110,7 @@ def decode_attention(q, cache: KVCache, lengths, counts=None, prefix: Optional[K
     share; its keys are read once for the whole batch.  Causal, with an optional
     window counted over prefix and own tokens.  Returns ``[B, S, Nq, H]`` in q's
     type; queries past ``counts`` give 0."""
-    from .kv_cache import decode_attention as f
-    return f(q, cache, lengths, counts, prefix, window, scale)
+    return _kv.decode_attention(q, cache, lengths, counts, prefix, window, scale)
 
 
 def verify_draft(target_logits, draft_tokens, uniform, noise, draft_logits=None, draft_lens=None, temperature=1.0):
@@ -128,8 +127,7 @@ def verify_draft(target_logits, draft_tokens, uniform, noise, draft_logits=None,
     ``accepted [B]`` and ``logp [B, K + 1]``, the log probability of each
     emitted token under the target at that temperature (0 where greedy).  NaN
     logits count as minus infinity; a row with none left yields token -1."""
-    from .spec import verify_draft as f
-    return f(target_logits, draft_tokens, uniform, noise, draft_logits, draft_lens, temperature)
+    return _spec.verify_draft(target_logits, draft_tokens, uniform, noise, draft_logits, draft_lens, temperature)
 
 
 # ------------------------------------------------------------------ swiglu

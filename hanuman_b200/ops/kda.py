@@ -14,7 +14,9 @@ import os
 
 import torch
 
+from . import reference as ref
 from ._ext import ext
+from .kv_cache import _int32, _need, _no_grad
 from .dense import _bf16, _gemm_or_narrow, _work, linear_fused, main_grad
 
 
@@ -98,38 +100,22 @@ def kda_chunked_cuda(q, k, v, g, beta, scale, chunk=None):
     return KdaCoreFn.apply(q, k, v, g, beta, scale)
 
 
-def _rows(t):
-    """Rows readable with any outer strides: only the last dimension is contiguous."""
-    return t if t.stride(-1) == 1 else t.contiguous()
-
-
 def kda_recurrent(q, k, v, g, beta, scale=None, state=None, counts=None):
     """The recurrence of :func:`hanuman_b200.ops.kda_recurrent` (csrc/serve/kda_recurrent.cu)."""
-    from .kv_cache import _int32, _need, _no_grad
+    if q.is_cuda:
+        return ext().kda_recurrent(q, k, v, g, beta, scale, state, counts)
     _need(q.dim() == 4 and q.shape == k.shape == v.shape == g.shape and q.shape[:3] == beta.shape,
           "kda_recurrent: q, k, v, g [B, S, H, K] and beta [B, S, H]")
     B, S, H, K = q.shape
     device = q.device
     _need(all(t.device == device for t in (k, v, g, beta)), "kda_recurrent: all inputs on one device")
-    scale = 1.0 / math.sqrt(K) if scale is None else float(scale)
     if state is not None:
         _need(state.dim() == 4 and state.shape[0] in (1, B) and state.shape[1:] == (H, K, K)
               and state.device == device and state.dtype == torch.float32,
               f"kda_recurrent: state [{B} or 1, {H}, {K}, {K}] fp32")
     _no_grad("kda_recurrent", q, k, v, g, beta, state)
     counts = None if counts is None else _int32(counts, "kda_recurrent: counts", B, device)
-    if not q.is_cuda:
-        from . import reference as ref
-        return ref.kda_recurrent_ragged(q, k, v, g, beta, scale, state, counts)
-    _need(q.dtype == k.dtype == v.dtype and q.dtype in (torch.float32, torch.bfloat16)
-          and g.dtype == beta.dtype == torch.float32, "kda_recurrent: fp32 or bf16 q, k, v; fp32 g and beta")
-    _need(K in (16, 32, 64, 128), f"kda_recurrent: head dim {K} is not 16, 32, 64 or 128")
-    if state is not None and B and not (state[0].is_contiguous() and state.stride(0) % 4 == 0 and state.data_ptr() % 16 == 0):
-        state = state.clone(memory_format=torch.contiguous_format)   # 16-byte loads
-    o = torch.empty(B, S, H, K, dtype=torch.float32, device=device)
-    new = torch.empty(B, H, K, K, dtype=torch.float32, device=device)
-    ext().kda_recurrent(_rows(q), _rows(k), _rows(v), _rows(g), beta, scale, state, counts, o, new)
-    return o, new
+    return ref.kda_recurrent_ragged(q, k, v, g, beta, scale, state, counts)
 
 
 class KdaFrontFn(torch.autograd.Function):

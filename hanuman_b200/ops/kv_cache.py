@@ -8,8 +8,8 @@ e4m3 codes and one power-of-two exponent per row,
     e = clamp(ceil(log2(amax / 448)), -120, 119),   code = e4m3(x 2^-e),
 
 so the value ``code * 2^e`` is exact in bf16; a bf16 cache holds the rows
-themselves.  The functions here check their arguments; the public entry points
-are in :mod:`hanuman_b200.ops`.
+themselves.  Wrong arguments raise ValueError (on the GPU from the native entry,
+csrc/serve/checks.h).  The public entry points are in :mod:`hanuman_b200.ops`.
 """
 from __future__ import annotations
 
@@ -20,8 +20,6 @@ import torch
 
 from . import reference as ref
 from ._ext import ext
-
-HEAD_DIMS = (32, 64, 128)
 
 
 class KVCache(NamedTuple):
@@ -77,90 +75,74 @@ def _int32(x, name: str, batch: int, device) -> torch.Tensor:
     return x if x.dtype == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
 
 
-def check_cache(cache: KVCache, name: str, device):
+def _check_cache(cache: KVCache, name: str, device):
     k, v = cache.k, cache.v
     _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device == device,
           f"{name}: keys and values of one shape [B, C, N, H], type and device")
-    if cache.quantised:
+    if cache.k_exp is not None or cache.v_exp is not None:
         _need(k.dtype == torch.float8_e4m3fn, f"{name}: a cache with exponents holds float8_e4m3fn codes")
         for e in (cache.k_exp, cache.v_exp):
             _need(e is not None and e.dtype == torch.int8 and e.shape == k.shape[:3] and e.device == device,
-                  f"{name}: int8 exponents [B, C, N]")
+                  f"{name}: int8 exponents [B, C, N] of keys and values")
     else:
-        _need(cache.v_exp is None and k.dtype != torch.float8_e4m3fn, f"{name}: 8-bit codes need their exponents")
-    if k.is_cuda:
-        _need(cache.quantised or k.dtype == torch.bfloat16, f"{name}: bf16 or float8_e4m3fn on the GPU")
-        _need(k.shape[3] in HEAD_DIMS, f"{name}: head dim {k.shape[3]} is not one of {HEAD_DIMS}")
-        for t in (k, v):
-            _need(_aligned(t), f"{name}: contiguous rows at 16-byte multiples")
-
-
-def _take(t: torch.Tensor) -> torch.Tensor:
-    """``t`` if the kernels can read it in place, else an aligned copy (a view of
-    contiguous values at an odd address is copied too)."""
-    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
-
-
-def _aligned(t: torch.Tensor) -> bool:
-    es = t.element_size()
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(t.stride(i) * es % 16 == 0 for i in range(t.dim() - 1) if t.shape[i] > 1))
+        _need(k.dtype != torch.float8_e4m3fn, f"{name}: 8-bit codes need their exponents")
 
 
 def kv_cache_write(cache: KVCache, k, v, starts, counts=None):
     device = cache.k.device
-    check_cache(cache, "kv_cache_write: cache", device)
     B, C, N, H = cache.k.shape
+    if isinstance(starts, int):
+        starts = _int32(starts, "", B, device)
+    if cache.k.is_cuda:
+        return ext().kv_cache_write(*cache, k, v, starts, counts)
+    _check_cache(cache, "kv_cache_write: cache", device)
     _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device == device
           and k.shape[0] == B and k.shape[2:] == (N, H),
           f"kv_cache_write: keys and values [{B}, S, {N}, {H}] of one type on {device}")
     _no_grad("kv_cache_write", k, v)
     starts = _int32(starts, "kv_cache_write: starts", B, device)
     counts = None if counts is None else _int32(counts, "kv_cache_write: counts", B, device)
-    if not k.is_cuda:
-        return ref.kv_cache_write(cache, k, v, starts, counts)
-    _need(k.dtype in (torch.bfloat16, torch.float32), "kv_cache_write: bf16 or fp32 rows")
-    k, v = _take(k), _take(v)
-    ext().kv_cache_write(k, v, cache.k, cache.v, cache.k_exp, cache.v_exp, starts, counts)
+    return ref.kv_cache_write(cache, k, v, starts, counts)
 
 
 def kv_cache_read(cache: KVCache, starts, n: int):
-    device = cache.k.device
-    check_cache(cache, "kv_cache_read: cache", device)
-    B, C, N, H = cache.k.shape
+    device, B = cache.k.device, cache.k.shape[0]
+    if isinstance(starts, int):
+        starts = _int32(starts, "", B, device)
+    if cache.k.is_cuda:
+        return ext().kv_cache_read(*cache, starts, n)
+    _check_cache(cache, "kv_cache_read: cache", device)
     _need(n >= 0, "kv_cache_read: n >= 0")
-    starts = _int32(starts, "kv_cache_read: starts", B, device)
-    if not cache.k.is_cuda:
-        return ref.kv_cache_read(cache, starts, n)
-    k, v = (torch.empty(B, n, N, H, dtype=torch.bfloat16, device=device) for _ in range(2))
-    ext().kv_cache_read(cache.k, cache.v, cache.k_exp, cache.v_exp, starts, k, v)
-    return k, v
+    return ref.kv_cache_read(cache, _int32(starts, "kv_cache_read: starts", B, device), n)
+
+
+_NO_PREFIX = (None,) * 4
 
 
 def decode_attention(q, cache: KVCache, lengths, counts=None, prefix: Optional[KVCache] = None, window: int = 0,
                      scale: Optional[float] = None):
+    if isinstance(lengths, int):
+        lengths = _int32(lengths, "", q.shape[0], q.device)
+    if isinstance(counts, int):
+        counts = _int32(counts, "", q.shape[0], q.device)
+    if q.is_cuda:
+        return ext().decode_attention(q, *cache, *(_NO_PREFIX if prefix is None else prefix), lengths, counts, window,
+                                      scale)
     device = q.device
     _need(q.dim() == 4, "decode_attention: q [B, S, Nq, H]")
     B, S, Nq, H = q.shape
-    check_cache(cache, "decode_attention: cache", device)
+    _check_cache(cache, "decode_attention: cache", device)
     N = cache.k.shape[2]
     _need(cache.k.shape[0] == B and cache.k.shape[3] == H and N > 0 and Nq % N == 0,
           f"decode_attention: a cache of {B} sequences, head dim {H} and KV heads that divide {Nq}")
     if prefix is not None:
-        check_cache(prefix, "decode_attention: prefix", device)
+        _check_cache(prefix, "decode_attention: prefix", device)
         _need(prefix.k.shape[0] == 1 and prefix.k.shape[2:] == (N, H) and prefix.k.dtype == cache.k.dtype,
               f"decode_attention: one prefix sequence [1, P, {N}, {H}] of the cache's type")
     _need(window >= 0, "decode_attention: window >= 0")
+    _need(scale is None or scale > 0, "decode_attention: scale > 0")
     _no_grad("decode_attention", q, cache.k, cache.v)
     lengths = _int32(lengths, "decode_attention: lengths", B, device)
     counts = None if counts is None else _int32(counts, "decode_attention: counts", B, device)
     scale = 1.0 / math.sqrt(H) if scale is None else float(scale)
-    if not q.is_cuda:
-        return ref.decode_attention(q, cache, lengths, counts, prefix, window, scale)
-    _need(q.dtype == torch.bfloat16, "decode_attention: bf16 queries on the GPU")
-    q = _take(q)
-    out = torch.empty(B, S, Nq, H, dtype=torch.bfloat16, device=device)
-    pk, pv, pke, pve = (None,) * 4 if prefix is None or prefix.capacity == 0 else prefix
-    ext().decode_attention(q, cache.k, cache.v, cache.k_exp, cache.v_exp, pk, pv, pke, pve, lengths, counts,
-                           int(window), scale, out)
-    return out
+    return ref.decode_attention(q, cache, lengths, counts, prefix, window, scale)

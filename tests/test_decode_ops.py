@@ -220,7 +220,7 @@ ATTN_SHAPES = [  # B, S, Nq, N, H, P, C
 
 @gpu
 @pytest.mark.parametrize("quant", [False, True])
-@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("window", [0, 1, 50])
 @pytest.mark.parametrize("shape", ATTN_SHAPES)
 def test_decode_attention_against_64_bits(shape, quant, window):
     B, S, Nq, N, H, P, C = shape
@@ -246,6 +246,10 @@ def test_decode_attention_long_keys_every_split(quant):
     q, cache, prefix, g = _attn_case(1, 1, 8, 2, 64, 5000, 20011, quant, dev="cuda")
     L = torch.tensor([20011], device="cuda")
     _attn_check(ops.decode_attention(q, cache, L, prefix=prefix), q, cache, L, None, prefix, 0)
+    for H, window in ((64, 0), (64, 700), (128, 0)):   # many rows: every CTA several tiles of two row blocks
+        q, cache, prefix, g = _attn_case(64, 4, 8, 2, H, 9001, 12, quant, dev="cuda")
+        L = torch.randint(4, 13, (64,), generator=g).cuda()
+        _attn_check(ops.decode_attention(q, cache, L, prefix=prefix, window=window), q, cache, L, None, prefix, window)
     q, cache, prefix, g = _attn_case(9, 2, 8, 2, 64, 0, 6000, quant, dev="cuda")
     L = torch.tensor([3, 6000, 2, 31, 32, 33, 64, 2, 5], device="cuda")
     _attn_check(ops.decode_attention(q, cache, L), q, cache, L, None, None, 0)
@@ -337,6 +341,7 @@ def test_decode_attention_refusals():
                 lambda: ops.decode_attention(q, cache, 1, prefix=other),           # another type
                 lambda: ops.decode_attention(q, cache, 1, prefix=cache),           # two sequences
                 lambda: ops.decode_attention(q, cache, 1, window=-1),
+                lambda: ops.decode_attention(q, cache, 1, scale=0.0),
                 lambda: ops.decode_attention(q.float().requires_grad_(), cache, 1),
                 lambda: ops.decode_attention(q[..., :32], cache, 1)):
         with pytest.raises(ValueError):
