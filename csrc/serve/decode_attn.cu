@@ -22,7 +22,7 @@
 // output (WHOLE).
 //
 // A CTA is 4 warps that share the rows and take every fourth 32-key tile, each
-// with its own cp.async ring, m, l and O (no barrier between tiles); they merge
+// with its own tiles, m, l and O (no barrier between tiles); they merge
 // through shared memory at the end of a piece.  Products on mma.sync: at S * G
 // rows the tensor work is small against the bytes of the keys.
 //
@@ -45,7 +45,7 @@ std::tuple<torch::Tensor, torch::Tensor> kv_cache_read(torch::Tensor k_cache, to
                                                        OptTensor v_exp, OptTensor starts, int64_t S);
 namespace {
 
-constexpr int WARPS = 4;
+constexpr int WARPS = 4;   // of a CTA that takes part of a sequence
 constexpr int KB = 32;   // keys per warp tile
 
 // 2^e for integers, 0 below the normal range.
@@ -75,17 +75,17 @@ HB_DEVICE PrePieces pre_pieces(const AttnParams& p, int n, int row) {
 }
 constexpr int MAX_PRE = 160;   // prefix pieces of a row
 
-template <int H, bool Q8, int MT>
+template <int H, bool Q8, int MT, int NW>
 struct Cfg {
   static constexpr int RB = Q8 ? H : 2 * H;             // bytes of a cached row
   static constexpr int CPR = RB / 16;                   // 16-byte chunks of it
   static constexpr int TILE = KB * RB;                  // K or V tile
-  static constexpr int ST = Q8 ? 3 : 2;                 // ring stages
-  static constexpr int RING = ST * 2 * TILE;            // per warp
+  static constexpr int EXP = Q8 ? 5 * KB * 4 : 0;       // words that hold the exponents; 2^ek, ev, 2^ev per key
+  static constexpr int RING = 2 * TILE + EXP;           // per warp: one K tile, one V tile
   static constexpr int QF = MT * (H / 16) * 32 * 16;    // query fragments
-  static constexpr int MERGE = WARPS * MT * 16 * (H + 4) * 4;
+  static constexpr int MERGE = NW * MT * 16 * (H + 4) * 4;
   static constexpr int JOIN = MERGE + MT * 16 * MAX_PRE * 4;
-  static constexpr int BODY = WARPS * RING > JOIN ? WARPS * RING : JOIN;
+  static constexpr int BODY = NW * RING > JOIN ? NW * RING : JOIN;
   static constexpr int SMEM = QF + MT * 16 * 4 + BODY;
 };
 
@@ -100,9 +100,10 @@ HB_DEVICE int tile_off(int r, int c) {
   else return r * RB + (c << 4);
 }
 
-template <int H, bool Q8, int MT, bool WHOLE>
-__global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParams p) {
-  using F = Cfg<H, Q8, MT>;
+template <int H, bool Q8, int MT, bool WHOLE, int NW>
+__global__ void __launch_bounds__(NW * 32, NW == 8 && MT == 1 && H <= 64 ? 2 : 1) decode_attn_kernel(const AttnParams p) {
+  static_assert(WHOLE || NW == WARPS, "the join of split sequences counts on WARPS");
+  using F = Cfg<H, Q8, MT, NW>;
   constexpr int KS = H / 16;        // k16 steps of q.k
   constexpr int NT = KB / 8;        // score tiles of 8 keys
   constexpr int JN = H / 8;         // output tiles of 8 columns
@@ -138,9 +139,9 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
     c = x / p.N;
     // tiles of all sequences: total, and the sequence that holds this CTA's first tile
     const bool report = blockIdx.x == p.n_pre;
-    __shared__ int wsum[WARPS];
+    __shared__ int wsum[NW];
     int total = 0;
-    for (int b0 = 0; b0 < p.B; b0 += WARPS * 32) {
+    for (int b0 = 0; b0 < p.B; b0 += NW * 32) {
       int v = 0;
       if (b0 + tid < p.B) {
         const int l = len_of(p, b0 + tid, report);
@@ -158,10 +159,10 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
       int base = total;
       for (int w = 0; w < warp; ++w) base += wsum[w];
       if (report && b0 + tid < p.B) p.tile_start[b0 + tid] = base + s - v;
-      total += wsum[0] + wsum[1] + wsum[2] + wsum[3];
+      for (int w = 0; w < NW; ++w) total += wsum[w];
     }
     if (report && tid == 0) p.tile_start[p.B] = total;
-    const int per = max(WARPS, (total + p.n_suf - 1) / p.n_suf);
+    const int per = max(NW, (total + p.n_suf - 1) / p.n_suf);
     tile0 = min(c * per, total), tile1 = min(tile0 + per, total);
     if (tile0 >= tile1) return;
     // second walk: every warp finds the sequence by itself
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
   }
   if (!WHOLE && tile0 >= tile1) {
     if (is_pre) {   // an empty split still has its slot
-      for (int r = tid; r < MT * 16; r += WARPS * 32) {
+      for (int r = tid; r < MT * 16; r += NW * 32) {
         const int rr = rt * MT * 16 + r;
         if (rr < p.B * SG) {
           float* ml = p.pre_ml + (((long long)n * p.n_split + c) * p.B * SG + rr) * 2;
@@ -224,35 +225,56 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
     const int8_t* vebase = Q8 ? kv.ve + b * kv.veb + n * kv.ven : nullptr;
 
     // tile tb + warp + 4 j of the piece is this warp's j-th
-    const int mine = max(0, (te - tb - warp + WARPS - 1) / WARPS);
-    auto load = [&](int j) {
-      const int key0 = key_lo + (tb + warp + WARPS * j) * KB;
-      const uint32_t kd = ring + (j % F::ST) * 2 * F::TILE, vd = kd + F::TILE;
+    const int mine = max(0, (te - tb - warp + NW - 1) / NW);
+    const uint32_t kt = ring, vt = ring + F::TILE, et = ring + 2 * F::TILE;
+    // One K and one V tile per warp: the next K is fetched while the weights of
+    // this tile and its product with V are computed, the next V during the next
+    // scores; the other warps of the SM fill what is left of the latency.
+    constexpr int RSTEP = 32 / F::CPR;   // rows between a lane's 16-byte chunks
+    const int r0 = lane / F::CPR, ch = lane % F::CPR;
+    auto load_rows = [&](uint32_t dst, const uint8_t* base, long long stride, int j) {
+      const int key0 = key_lo + (tb + warp + NW * j) * KB;
+      const uint8_t* src = base + (long long)(key0 + r0) * stride + ch * 16;
 #pragma unroll
-      for (int i = 0; i < KB * F::CPR / 32; ++i) {
-        const int x = i * 32 + lane, r = x / F::CPR, ch = x % F::CPR;
+      for (int i = 0; i < KB / RSTEP; ++i) {
+        const int r = r0 + i * RSTEP;
         const bool in = key0 + r < key_end;
-        const long long key = in ? key0 + r : key_lo;
-        cp_async16(kd + tile_off<H, Q8>(r, ch), kbase + key * kv.ks + ch * 16, in);
-        cp_async16(vd + tile_off<H, Q8>(r, ch), vbase + key * kv.vs + ch * 16, in);
+        cp_async16(dst + tile_off<H, Q8>(r, ch), in ? src : base + (long long)key_lo * stride, in);
+        src += RSTEP * stride;
       }
     };
-    int ex_next = 0;   // this lane's key of the next tile: key exponent in the low byte, value exponent above
-    auto load_exps = [&](int j) {
-      const int key = key_lo + (tb + warp + WARPS * j) * KB + lane;
-      int ke = 0, ve = -128;
-      if (j < mine && key < key_end) ke = kebase[key * kv.kes], ve = vebase[key * kv.ves];
-      ex_next = (ke & 0xff) | (ve << 8);
-    };
-#pragma unroll
-    for (int j = 0; j < F::ST - 1; ++j) {
-      if (j < mine) load(j);
+    auto load_k = [&](int j) {
+      if (j < mine) {
+        load_rows(kt, kbase, kv.ks, j);
+        if constexpr (Q8) {   // the aligned 4-byte words that hold the exponents of this lane's key
+          const long long key = min(key_lo + (tb + warp + NW * j) * KB + lane, key_end - 1);
+          const uintptr_t ka = reinterpret_cast<uintptr_t>(kebase + key * kv.kes), va = reinterpret_cast<uintptr_t>(vebase + key * kv.ves);
+          cp_async4(et + lane * 4, reinterpret_cast<const void*>(ka & ~uintptr_t(3)));
+          cp_async4(et + KB * 4 + lane * 4, reinterpret_cast<const void*>(va & ~uintptr_t(3)));
+        }
+      }
       cp_async_commit();
-    }
-    if constexpr (Q8) load_exps(0);
+    };
+    auto load_v = [&](int j) {
+      if (j < mine) load_rows(vt, vbase, kv.vs, j);
+      cp_async_commit();
+    };
+    float* sE = reinterpret_cast<float*>(body + warp * F::RING + 2 * F::TILE) + 2 * KB;   // 2^ek, ev, 2^ev
+    auto spread_exps = [&](int j) {   // this lane's key's, for the whole warp
+      const long long key = key_lo + (tb + warp + NW * j) * KB + lane;
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(sE) - 2 * KB;
+      const int ks = (int)((reinterpret_cast<uintptr_t>(kebase) + key * kv.kes) & 3) * 8;
+      const int vs = (int)((reinterpret_cast<uintptr_t>(vebase) + key * kv.ves) & 3) * 8;
+      const int ek = (int)(int8_t)(w[lane] >> ks), ev = key < key_end ? (int)(int8_t)(w[KB + lane] >> vs) : -128;
+      sE[lane] = pow2c(ek);
+      sE[KB + lane] = (float)ev;
+      sE[2 * KB + lane] = pow2c(ev);
+    };
+    load_k(0);
+    load_v(0);
 
     // query fragments, each warp one 16-row tile
-    for (int mt = warp; mt < MT; mt += WARPS) {
+    for (int mt = warp; mt < MT; mt += NW) {
       const __nv_bfloat16* qrow[2];
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
@@ -352,14 +374,10 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
     }
 
     for (int j = 0; j < mine; ++j) {
-      cp_async_wait<F::ST - 2>();
-      __syncwarp();   // every lane's part of tile j has landed; tile j - 1 has been read
-      if (j + F::ST - 1 < mine) load(j + F::ST - 1);
-      cp_async_commit();
-      const int ex = ex_next;
-      if constexpr (Q8) load_exps(j + 1);
-      const uint32_t kt = ring + (j % F::ST) * 2 * F::TILE, vt = kt + F::TILE;
-      const int key0 = key_lo + (tb + warp + WARPS * j) * KB;
+      cp_async_wait<1>();
+      __syncwarp();   // every lane's part of K tile j has landed
+      const int key0 = key_lo + (tb + warp + NW * j) * KB;
+      if constexpr (Q8) spread_exps(j);
 
       float s[MT][NT][4];
 #pragma unroll
@@ -415,15 +433,21 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
         }
       }
 
-      // scores in the log2 domain; masked ones minus infinity
-      const bool edge = key0 < max_lo || key0 + KB > min_hi;
-      int ekv[NT][2];
+      __syncwarp();   // K tile j has been read (and the exponents are spread)
+      float ke[NT][2], ev[NT][2], wv[NT][2];   // 2^ek; ev and 2^ev
       if constexpr (Q8) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) ekv[i][x] = __shfl_sync(0xffffffffu, ex, 8 * i + 2 * t + x);
+        for (int i = 0; i < NT; ++i) {
+          const float2 x = *reinterpret_cast<const float2*>(sE + 8 * i + 2 * t);
+          const float2 y = *reinterpret_cast<const float2*>(sE + KB + 8 * i + 2 * t);
+          const float2 z = *reinterpret_cast<const float2*>(sE + 2 * KB + 8 * i + 2 * t);
+          ke[i][0] = x.x, ke[i][1] = x.y, ev[i][0] = y.x, ev[i][1] = y.y, wv[i][0] = z.x, wv[i][1] = z.y;
+        }
       }
+      load_k(j + 1);
+
+      // scores in the log2 domain; masked ones minus infinity
+      const bool edge = key0 < max_lo || key0 + KB > min_hi;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -431,22 +455,11 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             float v = s[mt][i][x] * qsc[mt][x >> 1];
-            if constexpr (Q8) v *= pow2c((int)(int8_t)(ekv[i][x & 1] & 0xff));
+            if constexpr (Q8) v *= ke[i][x & 1];
             const int key = key0 + 8 * i + 2 * t + (x & 1);
             if (edge && (key < lo[mt][x >> 1] || key >= hi[mt][x >> 1])) v = -INFINITY;
             s[mt][i][x] = v;
           }
-      float wv[NT][2], ev[NT][2];   // 2^e and e of the value rows
-      if constexpr (Q8) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int e = ekv[i][x] >> 8;
-            ev[i][x] = (float)e;
-            wv[i][x] = pow2c(e);
-          }
-      }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         // new maxima: m of the scores, mo of the scores plus value exponents (O's unit)
@@ -508,6 +521,8 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
           s[mt][i][0] = __uint_as_float(r0), s[mt][i][1] = __uint_as_float(r1);
         }
       }
+      cp_async_wait<1>();
+      __syncwarp();   // V tile j has landed
 #pragma unroll
       for (int k = 0; k < KB / 16; ++k) {
         uint4 a[MT];
@@ -557,6 +572,8 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
             }
         }
       }
+      __syncwarp();   // V tile j has been read
+      load_v(j + 1);
     }
     cp_async_wait<0>();
 
@@ -595,13 +612,13 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
       // all of the sequence's own keys are here: join them with the prefix pieces
       wait_previous();
       const int rows = min(SG - rt * MT * 16, MT * 16);
-      float* sW = reinterpret_cast<float*>(body) + WARPS * MT * 16 * LD;   // weights of the pieces, then 1 / l
+      float* sW = reinterpret_cast<float*>(body) + NW * MT * 16 * LD;   // weights of the pieces, then 1 / l
       // a warp per row: M over the warps and the prefix pieces, weights, 1 / l
-      for (int r = warp; r < rows; r += WARPS) {
+      for (int r = warp; r < rows; r += NW) {
         const int rr = rt * MT * 16 + r;
         const float* row = reinterpret_cast<const float*>(body) + r * LD;
         const PrePieces pre = p.P > 0 ? pre_pieces(p, n, b * SG + rr) : PrePieces{0, 0, 0};
-        float M = lane < WARPS ? row[lane * MT * 16 * LD + H] : -INFINITY;
+        float M = lane < NW ? row[lane * MT * 16 * LD + H] : -INFINITY;
         for (int x = lane; x < pre.n; x += 32) {
           const float mp = p.pre_ml[(pre.at + x * pre.step) * 2];
           M = fmaxf(M, mp);
@@ -609,7 +626,7 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
         M = warp_max(M);
         float l = 0.f;
         float* w = sW + r * MAX_PRE;
-        if (lane < WARPS) {
+        if (lane < NW) {
           const float x = M > -INFINITY ? ex2f(row[lane * MT * 16 * LD + H] - M) : 0.f;
           l = x * row[lane * MT * 16 * LD + H + 1];
           w[lane] = x;
@@ -618,13 +635,13 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
           const float2 ml = *reinterpret_cast<const float2*>(p.pre_ml + (pre.at + x * pre.step) * 2);
           const float e = M > -INFINITY ? ex2f(ml.x - M) : 0.f;
           l += e * ml.y;
-          w[WARPS + x] = e;
+          w[NW + x] = e;
         }
         l = warp_sum(l);
         if (lane == 0) w[MAX_PRE - 1] = l > 0.f && rr / p.G < cnt ? 1.f / l : 0.f;
       }
       __syncthreads();
-      for (int x = tid; x < rows * CL; x += WARPS * 32) {
+      for (int x = tid; x < rows * CL; x += NW * 32) {
         const int r = x / CL, ch = x % CL * 4, rr = rt * MT * 16 + r;
         const float* row = reinterpret_cast<const float*>(body) + r * LD + ch;
         const float* w = sW + r * MAX_PRE;
@@ -635,13 +652,13 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
         };
         if (inv > 0.f) {
 #pragma unroll
-          for (int y = 0; y < WARPS; ++y) add(w[y], *reinterpret_cast<const float4*>(row + y * MT * 16 * LD));
+          for (int y = 0; y < NW; ++y) add(w[y], *reinterpret_cast<const float4*>(row + y * MT * 16 * LD));
           if (p.P > 0) {
             const PrePieces pre = pre_pieces(p, n, b * SG + rr);
             const float4* src = reinterpret_cast<const float4*>(p.pre_o + pre.at * H + ch);
             const long long step = pre.step * (H / 4);
 #pragma unroll 8
-            for (int y = 0; y < pre.n; ++y) add(w[WARPS + y], src[y * step]);
+            for (int y = 0; y < pre.n; ++y) add(w[NW + y], src[y * step]);
           }
         }
         const int i = rr / p.G, h = n * p.G + rr % p.G;
@@ -650,17 +667,17 @@ __global__ void __launch_bounds__(WARPS * 32) decode_attn_kernel(const AttnParam
       }
       break;
     }
-    for (int x = tid; x < MT * 16 * CL; x += WARPS * 32) {
+    for (int x = tid; x < MT * 16 * CL; x += NW * 32) {
       const int r = x / CL, ch = x % CL * 4, rr = rt * MT * 16 + r;
       if (rr >= (is_pre ? p.B * SG : SG)) continue;
       const float* row = reinterpret_cast<const float*>(body) + r * LD;
-      float M = -INFINITY, wt[WARPS], lsum = 0.f;
+      float M = -INFINITY, wt[NW], lsum = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, row[w * MT * 16 * LD + H]);
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, row[w * MT * 16 * LD + H]);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       if (M > -INFINITY)
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
+        for (int w = 0; w < NW; ++w) {
           wt[w] = ex2f(row[w * MT * 16 * LD + H] - M);
           lsum += wt[w] * row[w * MT * 16 * LD + H + 1];
           const float4 v = *reinterpret_cast<const float4*>(row + w * MT * 16 * LD + ch);
@@ -763,21 +780,21 @@ __global__ void __launch_bounds__(128) decode_combine_kernel(const AttnParams p)
   }
 }
 
-template <int H, bool Q8, int MT, bool WHOLE>
+template <int H, bool Q8, int MT, bool WHOLE, int NW>
 void launch_attn(const AttnParams& p) {
-  constexpr int smem = Cfg<H, Q8, MT>::SMEM;
+  constexpr int smem = Cfg<H, Q8, MT, NW>::SMEM;
   static bool configured[64] = {};
   int dev = 0;
   HB_CUDA_CHECK(cudaGetDevice(&dev));
   if (!configured[dev & 63]) {
-    HB_CUDA_CHECK(cudaFuncSetAttribute(decode_attn_kernel<H, Q8, MT, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    HB_CUDA_CHECK(cudaFuncSetAttribute(decode_attn_kernel<H, Q8, MT, WHOLE, NW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     configured[dev & 63] = true;
   }
   const long long blocks = WHOLE ? (long long)p.B * p.N * p.own_rt : p.n_pre + (long long)p.n_suf * p.N * p.own_rt;
   HB_CHECK(blocks < (1ll << 31), "decode_attention: too many tiles");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(WARPS * 32);
+  cfg.blockDim = dim3(NW * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = cur_stream();
   cudaLaunchAttribute at{};
@@ -785,7 +802,7 @@ void launch_attn(const AttnParams& p) {
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = WHOLE && p.tc_ctas > 0 ? 1 : 0;   // starts while the prefix kernel ends
-  HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, decode_attn_kernel<H, Q8, MT, WHOLE>, p));
+  HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, decode_attn_kernel<H, Q8, MT, WHOLE, NW>, p));
 }
 
 template <int H>
@@ -870,6 +887,8 @@ torch::Tensor decode_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v
   // is long: it joins the prefix pieces itself (one launch less).  Not where
   // the prefix runs on mma.sync, in the same launch as the own keys.
   const bool whole = (!p.P || tc) && (long long)p.B * p.N * p.own_rt >= sms / 2 && p.C <= 2048;
+  // eight warps a CTA where four would take more than two tiles each
+  const bool wide = p.C > 256;
   // own keys: about two CTAs per SM, at least 8 tiles of the full capacity each
   const long long cap_tiles = (long long)p.B * ((p.C + KB - 1) / KB);
   p.n_suf = (int)std::max<long long>(1, std::min<long long>(2ll * sms / ((long long)p.N * p.own_rt), cap_tiles / 8));
@@ -906,17 +925,19 @@ torch::Tensor decode_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v
       prefix_tc_launch(p, (int)H, p.pre.k, p.pre.v, p.pre.ks, p.pre.kn, p.pre.vs, p.pre.vn);
     }
   }
-#define HB_ATTN2(HH, W)                                                                 \
+#define HB_ATTN2(HH, W, NW)                                                                 \
   do {                                                                                  \
-    if (q8) mt == 2 ? launch_attn<HH, true, 2, W>(p) : launch_attn<HH, true, 1, W>(p);  \
-    else mt == 2 ? launch_attn<HH, false, 2, W>(p) : launch_attn<HH, false, 1, W>(p);   \
+    if (q8) mt == 2 ? launch_attn<HH, true, 2, W, NW>(p) : launch_attn<HH, true, 1, W, NW>(p);  \
+    else mt == 2 ? launch_attn<HH, false, 2, W, NW>(p) : launch_attn<HH, false, 1, W, NW>(p);   \
   } while (0)
 #define HB_ATTN(HH)          \
   do {                       \
-    if (whole) {             \
-      HB_ATTN2(HH, true);    \
+    if (whole && wide) {     \
+      HB_ATTN2(HH, true, 8); \
+    } else if (whole) {      \
+      HB_ATTN2(HH, true, 4); \
     } else {                 \
-      HB_ATTN2(HH, false);   \
+      HB_ATTN2(HH, false, WARPS);   \
       launch_combine<HH>(p); \
     }                        \
   } while (0)

@@ -5,16 +5,25 @@
 // Every column of S evolves by itself, so a CTA owns VC columns of one (b, h)
 // and the columns need no exchange.  A column's K rows lie in RG lanes of one
 // warp, R rows each, in registers for the whole call: the state is read once and
-// written once whatever the number of tokens.  Token rows (q, k, e^g, v, beta)
-// are staged TC at a time in shared memory, the next TC already in registers.
+// written once whatever the number of tokens.  Token rows are staged TC at a time
+// in shared memory, the next TC already in registers.
 //
-// Bound: with one token the state traffic (8 K V bytes); with many tokens the
-// dependent chain of a token (R multiply-adds, two or three shuffles, R more).
+// Within the TC tokens the state is kept as S = diag(D_t) X, D_t = e^{g summed from
+// the first of them}, which takes the decay out of the state's loop:
+//   u = beta (v - beta (D k)^T X);   X <- X + (k / D) u^T;   o = scale (D q)^T X
+// three multiply-adds per element instead of four operations (each one
+// instruction for two rows), with D k, k / D and D q computed once per token while
+// staging.  D >= e^-30 there keeps 1 / D and X far from overflow; tokens that
+// decay more (any row of the head) take the loop with the decay in it.
+//
+// Bound: with few tokens the state traffic (8 K V bytes); with many the
+// multiply-adds (6 K V per token), or with few heads the dependent chain of a token.
 #include <torch/extension.h>
 
 #include "../common/host.h"
 #include "../common/sm100.cuh"
 #include "checks.h"
+#include "f32x2.cuh"
 
 namespace hb {
 namespace {
@@ -44,9 +53,12 @@ HB_DEVICE float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 template <int CPT>
 HB_DEVICE void ldc(const float* p, float (&x)[CPT]) {
-  if constexpr (CPT == 4) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  if constexpr (CPT >= 4) {
+#pragma unroll
+    for (int c = 0; c < CPT; c += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + c);
+      x[c] = v.x, x[c + 1] = v.y, x[c + 2] = v.z, x[c + 3] = v.w;
+    }
   } else if constexpr (CPT == 2) {
     const float2 v = *reinterpret_cast<const float2*>(p);
     x[0] = v.x, x[1] = v.y;
@@ -56,10 +68,124 @@ HB_DEVICE void ldc(const float* p, float (&x)[CPT]) {
 }
 template <int CPT>
 HB_DEVICE void stc(float* p, const float (&x)[CPT]) {
-  if constexpr (CPT == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-  else if constexpr (CPT == 2) *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
+  if constexpr (CPT >= 4) {
+#pragma unroll
+    for (int c = 0; c < CPT; c += 4) *reinterpret_cast<float4*>(p + c) = make_float4(x[c], x[c + 1], x[c + 2], x[c + 3]);
+  } else if constexpr (CPT == 2) *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
   else *p = x[0];
 }
+
+// Sums acc[c] over the RG lanes of a column group (lane bits CL, 2 CL, ..).
+template <int CPT, int CL>
+HB_DEVICE void sum_lanes(float (&acc)[CPT]) {
+#pragma unroll
+  for (int d = CL; d < 32; d <<= 1)
+#pragma unroll
+    for (int c = 0; c < CPT; ++c) acc[c] += __shfl_xor_sync(0xffffffffu, acc[c], d);
+}
+
+// Sums of CPT values over the RG lanes, spread: an exchange over lane bit D leaves
+// each lane half of its columns, until one is left (the other bits of the lane
+// group just add).  CPT = 8: the column is lane bits 16, 8, 4; CPT = 4: 16, 8;
+// CPT = 2: 16; CPT = 1: every lane has it.
+template <int CPT, int CL, int D = 16>
+HB_DEVICE float sum_scatter(const float (&s)[CPT], int lane) {
+  if constexpr (CPT == 1) {
+    float x = s[0];
+#pragma unroll
+    for (int d = CL; d <= D; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+  } else {
+    static_assert(D >= CL, "as many lanes as columns");
+    const bool hi = lane & D;
+    float x[CPT / 2];
+#pragma unroll
+    for (int c = 0; c < CPT / 2; ++c) {
+      x[c] = hi ? s[CPT / 2 + c] : s[c];
+      x[c] += __shfl_xor_sync(0xffffffffu, hi ? s[c] : s[CPT / 2 + c], D);
+    }
+    return sum_scatter<CPT / 2, CL, D / 2>(x, lane);
+  }
+}
+// The way back: every lane gets all CPT values that sum_scatter's lanes hold.
+template <int CPT, int D = 16>
+HB_DEVICE void gather(float x, float (&s)[CPT], int lane) {
+  if constexpr (CPT == 1) {
+    s[0] = x;
+  } else {
+    float y[CPT / 2];
+    gather<CPT / 2, D / 2>(x, y, lane);
+    const bool hi = lane & D;
+#pragma unroll
+    for (int c = 0; c < CPT / 2; ++c) {
+      const float z = __shfl_xor_sync(0xffffffffu, y[c], D);
+      s[c] = hi ? z : y[c];
+      s[CPT / 2 + c] = hi ? y[c] : z;
+    }
+  }
+}
+// The column that sum_scatter leaves in a lane, and whether this lane writes it.
+template <int CPT>
+HB_DEVICE int own_column(int lane) {
+  return CPT == 8 ? (lane >> 4) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1) : CPT == 4 ? (lane >> 4) * 2 + (lane >> 3 & 1)
+         : CPT == 2 ? lane >> 4 : 0;
+}
+template <int CPT, int CL>
+HB_DEVICE void store_out(float* ot, float x, int lane) {
+  constexpr int OWN = CPT == 8 ? 28 : CPT == 4 ? 24 : CPT == 2 ? 16 : 0;   // lane bits that name the column
+  constexpr int REST = 31 & ~(CL - 1) & ~OWN;                              // the other bits of the lane group
+  if ((lane & REST) == 0) ot[own_column<CPT>(lane)] = x;
+}
+// Dot products of CPT columns' R rows with one staged row, or with two in one pass.
+template <int R, int CPT>
+HB_DEVICE void dot(const uint64_t (&st)[R / 2][CPT], const ulonglong2* a2, float (&s)[CPT]) {
+  uint64_t acc[CPT];
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) acc[c] = 0;
+#pragma unroll
+  for (int r = 0; r < R / 4; ++r) {
+    const ulonglong2 a = a2[r];
+#pragma unroll
+    for (int c = 0; c < CPT; ++c) acc[c] = fma2(st[2 * r + 1][c], a.y, fma2(st[2 * r][c], a.x, acc[c]));
+  }
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) {
+    float x, y;
+    unpack2(acc[c], x, y);
+    s[c] = x + y;
+  }
+}
+template <int R, int CPT>
+HB_DEVICE void dot2(const uint64_t (&st)[R / 2][CPT], const ulonglong2* a2, const ulonglong2* b2, float (&s)[CPT],
+                    float (&z)[CPT]) {
+  uint64_t as[CPT], az[CPT];
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) as[c] = az[c] = 0;
+#pragma unroll
+  for (int r = 0; r < R / 4; ++r) {
+    const ulonglong2 a = a2[r], b = b2[r];
+#pragma unroll
+    for (int c = 0; c < CPT; ++c) {
+      as[c] = fma2(st[2 * r][c], a.x, as[c]);
+      az[c] = fma2(st[2 * r][c], b.x, az[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < CPT; ++c) {
+      as[c] = fma2(st[2 * r + 1][c], a.y, as[c]);
+      az[c] = fma2(st[2 * r + 1][c], b.y, az[c]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CPT; ++c) {
+    float x, y;
+    unpack2(as[c], x, y);
+    s[c] = x + y;
+    unpack2(az[c], x, y);
+    z[c] = x + y;
+  }
+}
+
+constexpr float MIN_LOG_D = -30.f;   // least log D of the loop without decay
 
 // K rows, RG lanes per column group of CPT columns, VC columns per CTA, TC
 // staged tokens.
@@ -70,9 +196,11 @@ __global__ void __launch_bounds__(VC / CPT * RG) kda_recurrent_kernel(const RecP
   constexpr int CL = 32 / RG;               // column groups per warp
   constexpr int SEG = R + 4;                // padded rows of one lane group: distinct banks per group
   constexpr int ROW = RG * SEG;
-  constexpr int NE = (TC * K + THREADS - 1) / THREADS;   // staged q (k, g) elements per thread
+  constexpr int PARTS = THREADS / K;        // staging threads per row, TC / PARTS tokens each
+  constexpr int TP = TC / PARTS;
   constexpr int NV = (TC * VC + THREADS - 1) / THREADS;
-  __shared__ __align__(16) float sq[TC * ROW], sk[TC * ROW], sa[TC * ROW];
+  static_assert(THREADS % K == 0 && TC % PARTS == 0, "staging covers every row and token once");
+  __shared__ __align__(16) float sq[TC * ROW], sk[TC * ROW], sw[TC * ROW], sd[ROW];
   __shared__ __align__(16) float sv[TC * VC];
   __shared__ float sb[TC];
 
@@ -85,14 +213,14 @@ __global__ void __launch_bounds__(VC / CPT * RG) kda_recurrent_kernel(const RecP
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
   const int col = slice * VC + c0;
 
-  float st[R][CPT];
+  uint64_t st[R / 2][CPT];   // rows 2 r, 2 r + 1 of a column
   const float* s0 = p.s0 ? p.s0 + b * p.s0_b + ((long long)h * K + rg * R) * K + col : nullptr;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    if (s0) ldc<CPT>(s0 + r * K, st[r]);
-    else
+  for (int r = 0; r < R / 2; ++r) {
+    float x[CPT] = {}, y[CPT] = {};
+    if (s0) ldc<CPT>(s0 + 2 * r * K, x), ldc<CPT>(s0 + (2 * r + 1) * K, y);
 #pragma unroll
-      for (int c = 0; c < CPT; ++c) st[r][c] = 0.f;
+    for (int c = 0; c < CPT; ++c) st[r][c] = pack2(x[c], y[c]);
   }
 
   int n = p.S;
@@ -101,23 +229,24 @@ __global__ void __launch_bounds__(VC / CPT * RG) kda_recurrent_kernel(const RecP
     n = min(max(c, 0), p.S);
     if (c != n && tid == 0) set_error(p.status, kErrBounds);
   }
-  const T* q = reinterpret_cast<const T*>(p.q) + b * p.qs.b + h * p.qs.h;
-  const T* k = reinterpret_cast<const T*>(p.k) + b * p.ks.b + h * p.ks.h;
+  const int row = tid % K, part = tid / K;   // what this thread stages
+  const T* q = reinterpret_cast<const T*>(p.q) + b * p.qs.b + h * p.qs.h + row;
+  const T* k = reinterpret_cast<const T*>(p.k) + b * p.ks.b + h * p.ks.h + row;
   const T* v = reinterpret_cast<const T*>(p.v) + b * p.vs.b + h * p.vs.h + slice * VC;
-  const float* g = p.g + b * p.gs.b + h * p.gs.h;
+  const float* g = p.g + b * p.gs.b + h * p.gs.h + row;
   const float* be = p.beta + b * p.bs.b + h * p.bs.h;
   float* o = p.o + ((long long)b * p.S * p.H + h) * K + slice * VC;
 
-  float rq[NE], rk[NE], ra[NE], rv[NV], rb = 0.f;
+  float rq[TP], rk[TP], rgate[TC], rv[NV], rb = 0.f;
   auto fetch = [&](int t0) {
 #pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      const int idx = e * THREADS + tid, t = t0 + idx / K, i = idx % K;
-      const bool in = (TC * K % THREADS == 0 || idx < TC * K) && t < n;
-      rq[e] = in ? to_f(q[t * p.qs.s + i]) : 0.f;
-      rk[e] = in ? to_f(k[t * p.ks.s + i]) : 0.f;
-      ra[e] = in ? g[t * p.gs.s + i] : 0.f;
+    for (int e = 0; e < TP; ++e) {
+      const int t = t0 + part * TP + e;
+      rq[e] = t < n ? to_f(q[t * p.qs.s]) : 0.f;
+      rk[e] = t < n ? to_f(k[t * p.ks.s]) : 0.f;
     }
+#pragma unroll
+    for (int t = 0; t < TC; ++t) rgate[t] = t < (part + 1) * TP && t0 + t < n ? g[(t0 + t) * p.gs.s] : 0.f;
 #pragma unroll
     for (int e = 0; e < NV; ++e) {
       const int idx = e * THREADS + tid, t = t0 + idx / VC;
@@ -125,86 +254,135 @@ __global__ void __launch_bounds__(VC / CPT * RG) kda_recurrent_kernel(const RecP
     }
     rb = tid < TC && t0 + tid < n ? be[(t0 + tid) * p.bs.s] : 0.f;
   };
-  auto stage = [&]() {
+
+  if (n > 0) fetch(0);
+  for (int t0 = 0; t0 < n; t0 += TC) {
+    // log D of this thread's tokens (tokens past n have g = 0)
+    float cum = 0.f, ld[TP];
 #pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      const int idx = e * THREADS + tid;
-      if (TC * K % THREADS == 0 || idx < TC * K) {
-        const int t = idx / K, i = idx % K, at = t * ROW + i / R * SEG + i % R;
-        sq[at] = rq[e] * p.scale;
-        sk[at] = rk[e];
-        sa[at] = expf(ra[e]);
+    for (int t = 0; t < TC; ++t) {
+      cum += rgate[t];
+#pragma unroll
+      for (int e = 0; e < TP; ++e)
+        if (t == part * TP + e) ld[e] = cum;
+    }
+    // (the barrier also: the previous tokens have been used)
+    // (with one or two tokens there is nothing to gain: the short loop)
+    const bool in_loop = __syncthreads_or(!(cum >= MIN_LOG_D)) || TC <= 2;
+    const int at = row / R * SEG + row % R;
+#pragma unroll
+    for (int e = 0; e < TP; ++e) {
+      const int t = part * TP + e;
+      const float qe = rq[e] * p.scale;
+      if (!in_loop) {
+        const float d = expf(ld[e]);
+        sq[t * ROW + at] = qe * d;
+        sk[t * ROW + at] = rk[e] * d;
+        sw[t * ROW + at] = rk[e] * expf(-ld[e]);
+      } else {
+        float gt = 0.f;
+#pragma unroll
+        for (int x = 0; x < TC; ++x)
+          if (x == t) gt = rgate[x];
+        sq[t * ROW + at] = qe;
+        sk[t * ROW + at] = rk[e];
+        sw[t * ROW + at] = expf(gt);
       }
     }
+    if (part == PARTS - 1) sd[at] = expf(cum);
 #pragma unroll
     for (int e = 0; e < NV; ++e) {
       const int idx = e * THREADS + tid;
       if (TC * VC % THREADS == 0 || idx < TC * VC) sv[idx] = rv[e];
     }
     if (tid < TC) sb[tid] = rb;
-  };
-
-  if (n > 0) fetch(0);
-  for (int t0 = 0; t0 < n; t0 += TC) {
-    __syncthreads();   // the previous tokens have been used
-    stage();
     __syncthreads();
     if (t0 + TC < n) fetch(t0 + TC);
     const int tn = min(TC, n - t0);
-    for (int t = 0; t < tn; ++t) {
-      float kk[R], acc[CPT];
-      const float4* k4 = reinterpret_cast<const float4*>(sk + t * ROW + rg * SEG);
-      const float4* a4 = reinterpret_cast<const float4*>(sa + t * ROW + rg * SEG);
-      const float4* q4 = reinterpret_cast<const float4*>(sq + t * ROW + rg * SEG);
+    float* ot = o + (long long)t0 * p.H * K + c0;   // row of token t
+    if (TC > 2 && !in_loop) {
+      // one pass over X for the read of token t and the output of token t - 1:
+      // their reductions overlap, and a token's chain has one of them
+      for (int t = 0; t < tn; ++t) {
+        const ulonglong2* k2 = reinterpret_cast<const ulonglong2*>(sk + t * ROW + rg * SEG);
+        const ulonglong2* w2 = reinterpret_cast<const ulonglong2*>(sw + t * ROW + rg * SEG);
+        const ulonglong2* q2 = reinterpret_cast<const ulonglong2*>(sq + max(t - 1, 0) * ROW + rg * SEG);
+        float s[CPT], x[CPT];
+        dot2<R, CPT>(st, k2, q2, s, x);
+        const float beta = sb[t];
+        float y[CPT];
+        if constexpr (CPT == 8) {   // a lane makes one column's u, and they are handed round
+          const float r = sum_scatter<CPT, CL>(s, lane);
+          gather<CPT>(beta * (sv[t * VC + c0 + own_column<CPT>(lane)] - beta * r), y, lane);
+        } else {
+          sum_lanes<CPT, CL>(s);
 #pragma unroll
-      for (int c = 0; c < CPT; ++c) acc[c] = 0.f;
+          for (int c = 0; c < CPT; ++c) y[c] = beta * (sv[t * VC + c0 + c] - beta * s[c]);
+        }
+        const float out = sum_scatter<CPT, CL>(x, lane);
+        uint64_t u[CPT];
 #pragma unroll
-      for (int r = 0; r < R / 4; ++r) {
-        const float4 kv = k4[r], av = a4[r];
-        const float ks[4] = {kv.x, kv.y, kv.z, kv.w}, as[4] = {av.x, av.y, av.z, av.w};
+        for (int c = 0; c < CPT; ++c) u[c] = pack2(y[c], y[c]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          kk[4 * r + j] = ks[j];
+        for (int r = 0; r < R / 4; ++r) {
+          const ulonglong2 w = w2[r];
 #pragma unroll
-          for (int c = 0; c < CPT; ++c) {
-            st[4 * r + j][c] *= as[j];
-            acc[c] = fmaf(st[4 * r + j][c], ks[j], acc[c]);
-          }
+          for (int c = 0; c < CPT; ++c) st[2 * r][c] = fma2(w.x, u[c], st[2 * r][c]);
+#pragma unroll
+          for (int c = 0; c < CPT; ++c) st[2 * r + 1][c] = fma2(w.y, u[c], st[2 * r + 1][c]);
+        }
+        if (t > 0) {
+          store_out<CPT, CL>(ot, out, lane);
+          ot += (long long)p.H * K;
         }
       }
-#pragma unroll
-      for (int d = CL; d < 32; d <<= 1)
-#pragma unroll
-        for (int c = 0; c < CPT; ++c) acc[c] += __shfl_xor_sync(0xffffffffu, acc[c], d);
-      const float beta = sb[t];
-      float u[CPT], oa[CPT];
-#pragma unroll
-      for (int c = 0; c < CPT; ++c) {
-        u[c] = beta * (sv[t * VC + c0 + c] - beta * acc[c]);
-        oa[c] = 0.f;
-      }
+      float x[CPT];
+      dot<R, CPT>(st, reinterpret_cast<const ulonglong2*>(sq + (tn - 1) * ROW + rg * SEG), x);
+      store_out<CPT, CL>(ot, sum_scatter<CPT, CL>(x, lane), lane);
+      const ulonglong2* d2 = reinterpret_cast<const ulonglong2*>(sd + rg * SEG);   // S = diag(D) X
 #pragma unroll
       for (int r = 0; r < R / 4; ++r) {
-        const float4 qv = q4[r];
-        const float qs[4] = {qv.x, qv.y, qv.z, qv.w};
+        const ulonglong2 d = d2[r];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int c = 0; c < CPT; ++c) {
-            st[4 * r + j][c] = fmaf(kk[4 * r + j], u[c], st[4 * r + j][c]);
-            oa[c] = fmaf(st[4 * r + j][c], qs[j], oa[c]);
-          }
+        for (int c = 0; c < CPT; ++c) st[2 * r][c] = mul2(st[2 * r][c], d.x), st[2 * r + 1][c] = mul2(st[2 * r + 1][c], d.y);
       }
+    } else {
+      for (int t = 0; t < tn; ++t, ot += (long long)p.H * K) {
+        const ulonglong2* k2 = reinterpret_cast<const ulonglong2*>(sk + t * ROW + rg * SEG);
+        const ulonglong2* a2 = reinterpret_cast<const ulonglong2*>(sw + t * ROW + rg * SEG);
 #pragma unroll
-      for (int d = CL; d < 32; d <<= 1)
+        for (int r = 0; r < R / 4; ++r) {
+          const ulonglong2 a = a2[r];
 #pragma unroll
-        for (int c = 0; c < CPT; ++c) oa[c] += __shfl_xor_sync(0xffffffffu, oa[c], d);
-      if (rg == 0) stc<CPT>(o + (long long)(t0 + t) * p.H * K + c0, oa);
+          for (int c = 0; c < CPT; ++c) st[2 * r][c] = mul2(st[2 * r][c], a.x), st[2 * r + 1][c] = mul2(st[2 * r + 1][c], a.y);
+        }
+        float s[CPT];
+        dot<R, CPT>(st, k2, s);
+        sum_lanes<CPT, CL>(s);
+        const float beta = sb[t];
+#pragma unroll
+        for (int c = 0; c < CPT; ++c) {
+          const float y = beta * (sv[t * VC + c0 + c] - beta * s[c]);
+          const uint64_t u = pack2(y, y);
+#pragma unroll
+          for (int r = 0; r < R / 4; ++r) {
+            const ulonglong2 w = k2[r];
+            st[2 * r][c] = fma2(w.x, u, st[2 * r][c]), st[2 * r + 1][c] = fma2(w.y, u, st[2 * r + 1][c]);
+          }
+        }
+        dot<R, CPT>(st, reinterpret_cast<const ulonglong2*>(sq + t * ROW + rg * SEG), s);
+        store_out<CPT, CL>(ot, sum_scatter<CPT, CL>(s, lane), lane);
+      }
     }
   }
   float* s1 = p.s1 + (bh * K + rg * R) * K + col;
 #pragma unroll
-  for (int r = 0; r < R; ++r) stc<CPT>(s1 + r * K, st[r]);
+  for (int r = 0; r < R / 2; ++r) {
+    float x[CPT], y[CPT];
+#pragma unroll
+    for (int c = 0; c < CPT; ++c) unpack2(st[r][c], x[c], y[c]);
+    stc<CPT>(s1 + 2 * r * K, x), stc<CPT>(s1 + (2 * r + 1) * K, y);
+  }
   // tokens past the sequence's count have output 0
   for (int idx = tid; idx < (p.S - n) * VC; idx += THREADS)
     o[(long long)(n + idx / VC) * p.H * K + idx % VC] = 0.f;
@@ -220,15 +398,26 @@ void launch_rec(const RecParams& p) {
 
 template <typename T>
 void dispatch_rec(const RecParams& p, int K) {
-  if (p.S <= 8) {   // bound by the state's traffic: wide columns, one pass over few tokens
+  // Many heads: several columns per lane (the fewest instructions and shared-memory
+  // reads per element).  Few heads: the chain of a token counts, and one column
+  // per lane gives more and shorter ones.  On a B200, 16 heads x 256 tokens:
+  // K = 64, batch 8 (256 warps of the first kind) 101 against 70 us, 16 103 against
+  // 110, 32 151 against 190; K = 128, batch 8 (512 warps) 148 against 211.
+  const long long warps = (long long)p.B * p.H * K / 32;
+  if (p.S <= 2) {   // one or two tokens: the state's traffic
     if (K == 16) launch_rec<T, 16, 4, 2, 16, 2>(p);
     else if (K == 32) launch_rec<T, 32, 4, 4, 32, 2>(p);
     else if (K == 64) launch_rec<T, 64, 4, 4, 64, 2>(p);
-    else launch_rec<T, 128, 8, 4, 64, 2>(p);
+    else launch_rec<T, 128, 8, 4, 128, 2>(p);
+  } else if (warps >= 3ll * num_sms() || p.S <= 8) {
+    if (K == 16) launch_rec<T, 16, 4, 2, 16, 8>(p);
+    else if (K == 32) launch_rec<T, 32, 4, 4, 32, 8>(p);
+    else if (K == 64) launch_rec<T, 64, 4, 4, 64, 8>(p);
+    else launch_rec<T, 128, 8, 8, 128, 8>(p);
   } else {
-    if (K == 16) launch_rec<T, 16, 4, 1, 16, 16>(p);
-    else if (K == 32) launch_rec<T, 32, 4, 1, 32, 16>(p);
-    else if (K == 64) launch_rec<T, 64, 4, 1, 32, 16>(p);
+    if (K == 16) launch_rec<T, 16, 4, 1, 16, 8>(p);
+    else if (K == 32) launch_rec<T, 32, 4, 1, 32, 8>(p);
+    else if (K == 64) launch_rec<T, 64, 4, 1, 32, 8>(p);
     else launch_rec<T, 128, 8, 1, 32, 8>(p);
   }
 }

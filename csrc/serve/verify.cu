@@ -13,10 +13,10 @@
 //
 // One cluster of CTAs per sequence, each CTA a slice of the vocabulary: it reads
 // its slice of every row once, keeping the running maximum and sum of the
-// softmax (per thread, then per CTA), the cluster exchanges the (max, sum) pairs
-// through distributed shared memory, every CTA decides n alike, and the race
-// over row n reads that one row again (from L2) with the noise, which is
-// prefetched into L2 at the start.  One launch, no workspace.
+// softmax (per thread, then per CTA), every CTA writes its (max, sum) pairs into
+// its peers' shared memory, every CTA decides n alike, and the race over row n
+// reads that one row again (from L2) with the noise, which is prefetched into L2
+// at the start.  One launch, no workspace.
 //
 // Bound by memory: 2 K + 1 rows of V logits and one row of noise per sequence.
 #include <torch/extension.h>
@@ -24,13 +24,13 @@
 #include "../common/host.h"
 #include "../common/sm100.cuh"
 #include "checks.h"
+#include "f32x2.cuh"
 
 namespace hb {
 namespace {
 
-constexpr int VTHREADS = 512;
-constexpr int VWARPS = VTHREADS / 32;
 constexpr int VMAXROWS = 65;   // 2 K + 1 with K <= 32
+constexpr int VPIECES = 8;     // pieces of a row's slice, one warp each
 constexpr float LOG2E_F = 1.4426950408889634f;
 constexpr int NOIDX = 0x7fffffff;
 
@@ -100,56 +100,144 @@ HB_DEVICE Best warp_best(Best x) {
   return x;
 }
 
-// Calls vec(first index, values) for whole aligned 16-byte groups of row[c0, c1)
-// and one(index, value) for the ragged ends.
-template <typename T, int UNROLL, typename FV, typename F1>
-HB_DEVICE void for_slice(const T* row, int c0, int c1, FV vec, F1 one) {
+// A warp's share of one row: len logits from p (any alignment).  `ends(index,
+// value)` gets the ragged ends, at most one value per lane; then `batch(index of
+// the first group, values)` whole 16-byte groups, UNROLL at a time per lane (32
+// groups apart), all loaded before the first is used.  Groups past the end read
+// as minus infinity.
+template <typename T, int UNROLL, typename FE, typename FB>
+HB_DEVICE void for_logits(const T* p, int len, FE ends, FB batch) {
   constexpr int N = Vec<T>::N;
-  const int tid = threadIdx.x, len = c1 - c0;
-  if (len <= 0) return;
-  const T* p = row + c0;
+  const int lane = threadIdx.x & 31;
   const int mis = (int)((reinterpret_cast<uintptr_t>(p) / sizeof(T)) % N);
   const int head = min(len, mis ? N - mis : 0);
   const int nv = (len - head) / N, tail0 = head + nv * N;
-  if (tid < head) one(c0 + tid, logit_at(p, tid));
+  const int at = lane < head ? lane : 31 - lane < len - tail0 ? tail0 + 31 - lane : -1;
+  if (at >= 0) ends(at, logit_at(p, at));
   const uint4* pv = reinterpret_cast<const uint4*>(p + head);
-  int i = tid;
-  for (; i + (UNROLL - 1) * VTHREADS < nv; i += UNROLL * VTHREADS) {
+  const uint32_t none = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+  for (int i = lane; i < nv; i += UNROLL * 32) {
     uint4 u[UNROLL];
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j) u[j] = __ldg(pv + i + j * VTHREADS);
+    for (int j = 0; j < UNROLL; ++j) u[j] = __ldg(pv + min(i + j * 32, nv - 1));   // no branch between the loads
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j)
+      if (i + j * 32 >= nv) u[j] = make_uint4(none, none, none, none);
+    float f[UNROLL * N];
 #pragma unroll
     for (int j = 0; j < UNROLL; ++j) {
-      float f[N];
-      unpack(u[j], f, p);
-      vec(c0 + head + (i + j * VTHREADS) * N, f);
+      float g[N];
+      unpack(u[j], g, p);
+#pragma unroll
+      for (int k = 0; k < N; ++k) f[j * N + k] = g[k];
     }
+    batch(head + i * N, f);
   }
-  for (; i < nv; i += VTHREADS) {
-    float f[N];
-    unpack(__ldg(pv + i), f, p);
-    vec(c0 + head + i * N, f);
+}
+// Statistics of a warp's share.  The fast way takes every value as finite or
+// minus infinity; where a NaN or an infinity was among them its sum is NaN, and
+// the share is read again with them handled.
+template <typename T, int UNROLL>
+HB_DEVICE Stat warp_stat(const T* p, int len, float c) {
+  constexpr int NF = UNROLL * Vec<T>::N;
+  Stat st{-INFINITY, 0.f};
+  const auto start = [&](int, float x) {
+    if (x > -INFINITY) st = {x, 1.f};
+  };
+  for_logits<T, UNROLL>(p, len, start, [&](int, const float(&f)[NF]) {
+    float m = st.m, m2 = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NF; k += 4) m = max3(m, f[k], f[k + 1]), m2 = max3(m2, f[k + 2], f[k + 3]);
+    m = fmaxf(m, m2);
+    if (m > st.m) {
+      st.s *= vexp2((st.m - m) * c);   // 0 from the first maximum
+      st.m = m;
+    }
+    if (!(m > -INFINITY)) return;
+    const uint64_t nm = pack2(-m, -m), c2 = pack2(c, c);
+    uint64_t s0 = 0, s1 = 0;
+#pragma unroll
+    for (int k = 0; k < NF; k += 4) {
+      float x0, x1, x2, x3;
+      unpack2(mul2(add2(pack2(f[k], f[k + 1]), nm), c2), x0, x1);
+      unpack2(mul2(add2(pack2(f[k + 2], f[k + 3]), nm), c2), x2, x3);
+      s0 = add2(s0, pack2(vexp2(x0), vexp2(x1)));
+      s1 = add2(s1, pack2(vexp2(x2), vexp2(x3)));
+    }
+    float a, b;
+    unpack2(add2(s0, s1), a, b);
+    st.s += a + b;
+  });
+  if (__any_sync(0xffffffffu, st.s != st.s || st.m == INFINITY)) {
+    st = {-INFINITY, 0.f};
+    const auto one = [&](float x) {
+      x = as_logit(x);
+      st = merge(st, Stat{x, x > -INFINITY ? 1.f : 0.f}, c);
+    };
+    for_logits<T, UNROLL>(p, len, [&](int, float x) { one(x); }, [&](int, const float(&f)[NF]) {
+#pragma unroll 1
+      for (int j = 0; j < UNROLL; ++j)
+#pragma unroll
+        for (int k = 0; k < NF; ++k)
+          if (k / Vec<T>::N == j) one(f[k]);
+    });
   }
-  if (tid < len - tail0) one(c0 + tail0 + tid, logit_at(p, tail0 + tid));
+  const float m = warp_max(st.m);
+  const float s = warp_sum(m > -INFINITY ? st.s * ratio(st.m, m, c) : 0.f);
+  return {m, s};
+}
+// Greatest value of a warp's share and its lowest index (counted from `base`).
+template <typename T, int UNROLL>
+HB_DEVICE Best warp_argmax(const T* p, int len, int base) {
+  constexpr int N = Vec<T>::N, NF = UNROLL * N;
+  Best best{-INFINITY, NOIDX};
+  const auto one = [&](int i, float x) {
+    if (x > best.v || (x == best.v && x > -INFINITY && base + i < best.i)) best = {x, base + i};
+  };
+  for_logits<T, UNROLL>(p, len, one, [&](int i, const float(&f)[NF]) {
+    float m = max3(f[0], f[1], f[2]);
+#pragma unroll
+    for (int k = 3; k + 1 < NF; k += 2) m = max3(m, f[k], f[k + 1]);
+    m = fmaxf(m, f[NF - 1]);
+    if (m >= best.v) {   // seldom after the first values
+#pragma unroll
+      for (int k = 0; k < NF; ++k) one(i + k / N * 32 * N + k % N, f[k]);
+    }
+  });
+  return warp_best(best);
 }
 
-HB_DEVICE float dsmem_f32(uint32_t addr, uint32_t rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(addr, rank)));
-  return v;
+// The cluster's CTAs have to have started before one writes to another's shared
+// memory: arrive at the start, wait before the first such write.
+HB_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+HB_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// Writes two words at the same place of CTA `rank`'s shared memory.
+HB_DEVICE void push2(const void* at, uint32_t rank, uint32_t x, uint32_t y) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(mapa_shared(smem_u32(at), rank)), "r"(x), "r"(y) : "memory");
 }
-
+// Asks for [p, p + len) to be brought to L2.
 template <typename T>
-__global__ void __launch_bounds__(VTHREADS) verify_kernel(const VerifyParams p, const int cs) {
-  constexpr int N = Vec<T>::N;
-  __shared__ Stat part[VMAXROWS][VWARPS];   // per warp; then [.][0] is the CTA's
-  __shared__ Best bpart[VMAXROWS][VWARPS];
-  __shared__ Best rpart[2][VWARPS];         // of the race
-  __shared__ Stat full[VMAXROWS];           // of the whole rows
-  __shared__ int first[VMAXROWS];           // greedy: index of the row's maximum
-  __shared__ float fin[4];                  // race results of this CTA: (score, index) twice
-  __shared__ int s_n;
+HB_DEVICE void prefetch_l2(const T* p, int len) {
+  const uintptr_t a = (reinterpret_cast<uintptr_t>(p) + 15) & ~uintptr_t(15), b = reinterpret_cast<uintptr_t>(p + len) & ~uintptr_t(15);
+  if (b > a)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a), "r"((uint32_t)(b - a)) : "memory");
+}
+constexpr int MAX_CS = 8;   // CTAs of a cluster
 
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) verify_kernel(const VerifyParams p, const int cs) {
+  constexpr int VWARPS = NT / 32;
+  constexpr int VUNROLL = 32 / Vec<T>::N;   // 32 logits in flight per lane
+  __shared__ Stat part[VMAXROWS][VPIECES];       // per piece of this CTA's slice (greedy: value and index)
+  __shared__ __align__(8) Stat slices[MAX_CS][VMAXROWS];   // of every CTA's slice, written by its CTA
+  __shared__ __align__(8) Stat full[VMAXROWS];   // of the whole rows
+  __shared__ Best rpart[VWARPS];                 // of the race, per warp
+  __shared__ __align__(8) float fin[MAX_CS][2];  // of the race, per slice: score, index
+  __shared__ int s_n;
+  __shared__ float s_logit[32];                  // target logits of the drafted tokens
+  __shared__ int s_tok[32];                      // the drafted tokens
+
+  cluster_arrive();
   const int b = blockIdx.x / cs, rank = blockIdx.x % cs;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int V = p.V, K = p.K;
@@ -171,102 +259,84 @@ __global__ void __launch_bounds__(VTHREADS) verify_kernel(const VerifyParams p, 
   }
   const int nt = L + 1, rows = greedy || !dr ? nt : nt + L;   // row r < nt: target r, else draft r - nt
 
-  if (!greedy)   // the race reads this slice of the noise at the end: bring it to L2 now
-    for (int i = c0 + tid * 32; i < c1; i += VTHREADS * 32)
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(nz + i));
+  // what the acceptance needs of the drafted tokens is on its way from the start
+  float xt = -INFINITY, xd = -INFINITY, uni = 0.f;
+  long long drafted = -1;
+  bool valid = false;
+  if (warp == 0 && lane < L) {
+    drafted = p.tokens[(long long)b * K + lane];
+    uni = p.uniform[(long long)b * K + lane];
+    valid = index_ok(drafted, V, rank == 0 ? p.status : nullptr);
+    if (valid) {
+      xt = logit_at(tg, (long long)lane * V + drafted);
+      if (dr) xd = logit_at(dr, (long long)lane * V + drafted);
+    }
+  }
+  if (!greedy && warp == 1 && lane == 0) prefetch_l2(nz + c0, c1 - c0);   // read by the race at the end
 
-  for (int r = 0; r < rows; ++r) {
-    const T* row = r < nt ? tg + (long long)r * V : dr + (long long)(r - nt) * V;
+  // (row, piece of the slice) units, one warp each: the warps' loads overlap
+  // freely; there is no barrier between rows
+  const int slice = c1 - c0, pieces = min(VPIECES, max(1, (slice + 2047) / 2048));
+  const int plen = ((slice + pieces - 1) / pieces + 7) / 8 * 8;
+  const int units = rows * pieces;
+  const auto place = [&](int u, const T*& row, int& a, int& len) {
+    const int r = u / pieces, q = u % pieces;
+    a = min(slice, q * plen), len = min(slice, a + plen) - a;
+    row = (r < nt ? tg + (long long)r * V : dr + (long long)(r - nt) * V) + c0 + a;
+  };
+  const auto ahead = [&](int u) {   // this warp's next units are brought to L2 meanwhile
+    if (lane == 0 && u < units) {
+      const T* row;
+      int a, len;
+      place(u, row, a, len);
+      prefetch_l2(row, len);
+    }
+  };
+  ahead(warp + VWARPS);
+  for (int u = warp; u < units; u += VWARPS) {
+    ahead(u + 2 * VWARPS);
+    const T* row;
+    int a, len;
+    place(u, row, a, len);
+    const int r = u / pieces, q = u % pieces;
     if (greedy) {
-      Best best{-INFINITY, NOIDX};
-      auto one = [&](int i, float x) {
-        if (x > best.v || (x == best.v && x > -INFINITY && i < best.i)) best = {x, i};
-      };
-      for_slice<T, 4>(row, c0, c1,
-                      [&](int i, const float(&f)[N]) {
-#pragma unroll
-                        for (int j = 0; j < N; ++j) one(i + j, f[j]);
-                      },
-                      one);
-      best = warp_best(best);
-      if (lane == 0) bpart[r][warp] = best;
+      const Best best = warp_argmax<T, VUNROLL>(row, len, c0 + a);
+      if (lane == 0) part[r][q] = {best.v, __int_as_float(best.i)};
     } else {
-      Stat st{-INFINITY, 0.f};
-      auto one = [&](int, float x) { st = merge(st, Stat{x, x > -INFINITY ? 1.f : 0.f}, cexp); };
-      for_slice<T, 4>(row, c0, c1,
-                      [&](int, const float(&f)[N]) {
-                        float m = fmaxf(f[0], f[1]);   // fmaxf drops NaN
-#pragma unroll
-                        for (int j = 2; j < N; ++j) m = fmaxf(m, f[j]);
-                        if (m > st.m) {
-                          st.s *= vexp2((st.m - m) * cexp);   // 0 from the first maximum
-                          st.m = m;
-                        }
-                        if (st.m > -INFINITY) {
-#pragma unroll
-                          for (int j = 0; j < N; ++j) {
-                            const float e = f[j] == st.m ? 1.f : vexp2((f[j] - st.m) * cexp);
-                            st.s += f[j] == f[j] ? e : 0.f;
-                          }
-                        }
-                      },
-                      one);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-        st = merge(st, Stat{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o)}, cexp);
-      if (lane == 0) part[r][warp] = st;
+      const Stat st = warp_stat<T, VUNROLL>(row, len, cexp);
+      if (lane == 0) part[r][q] = st;
     }
   }
   __syncthreads();
-  for (int r = warp; r < rows; r += VWARPS) {
-    if (greedy) {
-      Best x = lane < VWARPS ? bpart[r][lane] : Best{-INFINITY, NOIDX};
-      x = warp_best(x);
-      __syncwarp();
-      if (lane == 0) bpart[r][0] = x;
-    } else {
-      Stat x = lane < VWARPS ? part[r][lane] : Stat{-INFINITY, 0.f};
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-        x = merge(x, Stat{__shfl_xor_sync(0xffffffffu, x.m, o), __shfl_xor_sync(0xffffffffu, x.s, o)}, cexp);
-      __syncwarp();
-      if (lane == 0) part[r][0] = x;
-    }
+  cluster_wait();
+  // a thread per (row, peer) joins the row's pieces and hands them to the peer
+  const auto join = [&](Stat x, Stat y) -> Stat {
+    if (!greedy) return merge(x, y, cexp);
+    const Best z = better(Best{x.m, __float_as_int(x.s)}, Best{y.m, __float_as_int(y.s)});
+    return {z.v, __int_as_float(z.i)};
+  };
+  for (int x = tid; x < rows * cs; x += NT) {
+    const int r = x / cs;
+    Stat y = part[r][0];
+    for (int q = 1; q < pieces; ++q) y = join(y, part[r][q]);
+    push2(&slices[rank][r], x % cs, __float_as_uint(y.m), __float_as_uint(y.s));
   }
   __syncwarp();
   cluster_sync_all();
-  for (int r = tid; r < rows; r += VTHREADS) {   // every CTA merges all slices in the same order
-    if (greedy) {
-      Best x{-INFINITY, NOIDX};
-      for (int c = 0; c < cs; ++c) {
-        const uint32_t a = smem_u32(&bpart[r][0]);
-        x = better(x, Best{dsmem_f32(a, c), __float_as_int(dsmem_f32(a + 4, c))});
-      }
-      first[r] = x.i;
-    } else {
-      Stat x{-INFINITY, 0.f};
-      for (int c = 0; c < cs; ++c) {
-        const uint32_t a = smem_u32(&part[r][0]);
-        x = merge(x, Stat{dsmem_f32(a, c), dsmem_f32(a + 4, c)}, cexp);
-      }
-      full[r] = x;
-    }
+  for (int r = tid; r < rows; r += NT) {   // every CTA joins all slices in the same order
+    Stat x = slices[0][r];
+    for (int c = 1; c < cs; ++c) x = join(x, slices[c][r]);
+    full[r] = x;
   }
   __syncthreads();
-  if (warp == 0) {   // acceptance, 32 drafted positions at a time (K <= 32)
+  if (warp == 0) {   // acceptance, a lane per drafted position (K <= 32)
     bool ok = false;
     if (lane < L) {
-      const long long x = p.tokens[(long long)b * K + lane];
-      if (index_ok(x, V, p.status)) {
-        if (greedy) {
-          ok = (int)x == first[lane];
-        } else {
-          const float pt = prob(logit_at(tg, (long long)lane * V + x), full[lane], inv);
-          float qt = 1.f;
-          if (dr) qt = prob(logit_at(dr, (long long)lane * V + x), full[nt + lane], inv);
-          ok = p.uniform[(long long)b * K + lane] * qt < pt;
-        }
+      if (valid) {
+        if (greedy) ok = (int)drafted == __float_as_int(full[lane].s);
+        else ok = uni * (dr ? prob(xd, full[nt + lane], inv) : 1.f) < prob(xt, full[lane], inv);
       }
+      s_logit[lane] = xt, s_tok[lane] = valid ? (int)drafted : -1;
     }
     const unsigned rej = ~__ballot_sync(0xffffffffu, ok);
     if (lane == 0) s_n = min(L, rej ? __ffs(rej) - 1 : 32);
@@ -274,86 +344,128 @@ __global__ void __launch_bounds__(VTHREADS) verify_kernel(const VerifyParams p, 
   __syncthreads();
   const int n = s_n;
 
-  // the race over row n: residual scores and, in case every residual is 0, p's own
-  Best res{0.f, NOIDX}, own{0.f, NOIDX};
-  if (!greedy) {
-    const Stat ft = full[n];
-    const bool minus = n < L;
-    const Stat fd = minus && dr ? full[nt + n] : Stat{0.f, 0.f};
-    const long long taken = minus && !dr ? p.tokens[(long long)b * K + n] : -1;
-    const T* trow = tg + (long long)n * V;
-    const T* drow = minus && dr ? dr + (long long)n * V : nullptr;
-    if (ft.s > 0.f)
-      for (int i = c0 + tid; i < c1; i += VTHREADS) {
-        const float pj = prob(logit_at(trow, i), ft, inv), e = nz[i];
-        float r = pj;
-        if (drow) r = fmaxf(pj - prob(logit_at(drow, i), fd, inv), 0.f);
-        if (i == taken) r = 0.f;
-        const float sr = r / e, so = pj / e;
-        if (sr > res.v) res = {sr, i};
-        if (so > own.v) own = {so, i};
+  // The race over row n.  Approximate exponentials and reciprocals bound each
+  // score from both sides (they are within 2^-17 of p down to p = 2^-126; the
+  // margin is 2^-16); only a logit whose upper bound reaches the best lower bound
+  // of the CTA, all but always one, is computed in full.  (An exact score costs
+  // some 1500 cycles, most of them three divisions; exact scores for each
+  // thread's, or even each warp's, own records took most of the race's time.)
+  const Stat ft = greedy ? Stat{0.f, 0.f} : full[n];
+  const bool minus = n < L;
+  const Stat fd = !greedy && minus && dr ? full[nt + n] : Stat{0.f, 0.f};
+  const long long taken = minus && !dr ? (long long)s_tok[n] : -1;
+  const T* trow = tg + (long long)n * V;
+  const T* drow = minus && dr && fd.s > 0.f ? dr + (long long)n * V : nullptr;
+  const auto race = [&](const T* dl, long long skip) {   // argmax of max(p - q, 0) / noise over this CTA's slice
+    const bool odd = ft.m == INFINITY || fd.m == INFINITY;   // no bounds there
+    constexpr float UP = 1.f + 0x1p-16f, DOWN = 1.f - 0x1p-16f;
+    const float it = 1.f / ft.s, id = dl ? 1.f / fd.s : 0.f;
+    float low = 0.f, top = 0.f, second = 0.f;   // of this thread: best lower bound, two best upper ones
+    int at = c0;
+    constexpr int RU = 8;   // logits in flight per thread
+    const T* dn = dl ? dl : trow;   // without a draft its share is multiplied by id = 0
+    const float dm = dl ? fd.m : ft.m;
+    for (int i0 = c0 + tid; i0 < c1; i0 += RU * NT) {
+      T xt[RU], xd[RU];
+      float e[RU];
+#pragma unroll
+      for (int j = 0; j < RU; ++j) {   // no branch and no use between the loads
+        const int i = min(i0 + j * NT, c1 - 1);
+        xt[j] = trow[i], xd[j] = dn[i], e[j] = nz[i];
       }
-  }
-  res = warp_best(res), own = warp_best(own);
-  if (lane == 0) rpart[0][warp] = res, rpart[1][warp] = own;
-  __syncthreads();
-  if (warp == 0) {
-    Best x = warp_best(lane < VWARPS ? rpart[0][lane] : Best{0.f, NOIDX});
-    Best y = warp_best(lane < VWARPS ? rpart[1][lane] : Best{0.f, NOIDX});
-    if (lane == 0) {
-      fin[0] = x.v, fin[1] = __int_as_float(x.i);
-      fin[2] = y.v, fin[3] = __int_as_float(y.i);
+#pragma unroll
+      for (int j = 0; j < RU; ++j) {
+        const int i = i0 + j * NT;
+        const float pa = vexp2((fmaxf((float)xt[j], -INFINITY) - ft.m) * cexp) * it;   // fmaxf: NaN as minus infinity
+        const float qa = vexp2((fmaxf((float)xd[j], -INFINITY) - dm) * cexp) * id;
+        const float w = i == skip || i >= c1 ? 0.f : __fdividef(1.f, e[j]);
+        const float up = fmaf(pa, UP, -qa * DOWN) * w * UP;
+        low = fmaxf(low, fmaf(pa, DOWN, -qa * UP) * w * DOWN);
+        second = fmaxf(second, fminf(top, up));
+        if (up > top) top = up, at = i;
+      }
     }
+    low = warp_max(low);
+    if (lane == 0) rpart[warp].v = low;
+    __syncthreads();
+    low = warp_max(lane < VWARPS ? rpart[lane].v : 0.f);
+    __syncthreads();
+    Best best{0.f, NOIDX};
+    const auto exact = [&](int i) {
+      float r = prob(logit_at(trow, i), ft, inv);
+      if (dl) r = fmaxf(r - prob(logit_at(dl, i), fd, inv), 0.f);
+      if (i == skip) r = 0.f;
+      const float s = r / nz[i];
+      if (s > best.v) best = {s, i};
+    };
+    if (odd || (second >= low && second > 0.f)) {   // two that may win in one thread: all of its logits
+      for (int i = c0 + tid; i < c1; i += NT) exact(i);
+    } else if (top >= low && top > 0.f) {
+      exact(at);
+    }
+    best = warp_best(best);
+    if (lane == 0) rpart[warp] = best;
+    __syncthreads();
+    if (warp == 0) {
+      best = warp_best(lane < VWARPS ? rpart[lane] : Best{0.f, NOIDX});
+      if (lane < cs) push2(fin[rank], lane, __float_as_uint(best.v), (uint32_t)best.i);
+    }
+    __syncwarp();
+    cluster_sync_all();
+    Best all{0.f, NOIDX};   // every CTA joins all slices alike
+    for (int c = 0; c < cs; ++c) all = better(all, Best{fin[c][0], __float_as_int(fin[c][1])});
+    return all;
+  };
+  int next = NOIDX;
+  if (greedy) {
+    next = __float_as_int(full[n].s);
+  } else if (ft.s > 0.f) {
+    Best x = race(drow, taken);
+    if (!(x.v > 0.f) && minus) {   // nothing left of p - q: p itself
+      __syncthreads();
+      cluster_sync_all();   // every CTA has read the first race's results
+      x = race(nullptr, -1);
+    }
+    next = x.i;
   }
-  __syncwarp();
-  cluster_sync_all();
+  // (no CTA writes to a peer's shared memory after the last cluster barrier)
   if (rank == 0 && warp == 0) {
-    int next;
-    if (greedy) {
-      next = first[n];
-    } else {
-      Best x{0.f, NOIDX}, y{0.f, NOIDX};
-      for (int c = 0; c < cs; ++c) {
-        const uint32_t a = smem_u32(fin);
-        x = better(x, Best{dsmem_f32(a, c), __float_as_int(dsmem_f32(a + 4, c))});
-        y = better(y, Best{dsmem_f32(a + 8, c), __float_as_int(dsmem_f32(a + 12, c))});
-      }
-      next = x.v > 0.f ? x.i : y.i;
-    }
+    const float xn = !greedy && next < V ? logit_at(trow, next) : 0.f;
     for (int i = lane; i <= K; i += 32) {
       long long tok = -1;
-      if (i < n) tok = p.tokens[(long long)b * K + i];
+      float x = xn;
+      if (i < n) tok = s_tok[i], x = s_logit[i];
       else if (i == n) tok = next < V ? next : -1;
       float lp = 0.f;
-      if (tok >= 0 && !greedy) {
-        const Stat f = full[i];
-        const float x = logit_at(tg, (long long)i * V + tok);
-        lp = (x == f.m ? 0.f : (x - f.m) * inv) - logf(f.s);
-      }
+      if (tok >= 0 && !greedy) lp = (x == full[i].m ? 0.f : (x - full[i].m) * inv) - logf(full[i].s);
       p.out[(long long)b * (K + 1) + i] = tok;
       p.logp[(long long)b * (K + 1) + i] = lp;
     }
     if (lane == 0) p.accepted[b] = n;
   }
-  __syncwarp();
-  cluster_sync_all();   // the peers' shared memory is read until here
 }
 
 template <typename T>
 void launch_verify(const VerifyParams& p) {
-  // Enough CTAs for two waves' worth of SMs, slices of at least 1024 logits.
-  int cs = 8;
+  // As many CTAs as the GPU holds at once (four of 256 threads an SM), with slices of at least
+  // 1024 logits; 8 CTAs (the portable cluster) at most: 16 took 13.5 us against 12.5
+  // for one sequence and 25 against 16 for 16 of them.
+  int cs = MAX_CS;
   while (cs > 1 && ((long long)p.B * cs > 4 * num_sms() || p.V / cs < 1024)) cs /= 2;
+  // 16 warps a CTA where one CTA per SM is about all there is, else 8: the phases
+  // of more CTAs overlap.
+  const bool wide = (long long)p.B * cs <= 2 * num_sms();
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)p.B * cs);
-  cfg.blockDim = dim3(VTHREADS);
+  cfg.blockDim = dim3(wide ? 512 : 256);
   cfg.stream = cur_stream();
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
   at.val.clusterDim.x = cs, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_kernel<T>, p, cs));
+  if (wide) HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_kernel<T, 512>, p, cs));
+  else HB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, verify_kernel<T, 256>, p, cs));
 }
 
 }  // namespace
