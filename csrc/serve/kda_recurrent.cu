@@ -190,7 +190,7 @@ constexpr float MIN_LOG_D = -30.f;   // least log D of the loop without decay
 // K rows, RG lanes per column group of CPT columns, VC columns per CTA, TC
 // staged tokens.
 template <typename T, int K, int RG, int CPT, int VC, int TC>
-__global__ void __launch_bounds__(VC / CPT * RG) kda_recurrent_kernel(const RecParams p) {
+__global__ void __launch_bounds__(VC / CPT * RG, TC <= 2 ? 512 / (VC / CPT * RG) : 1) kda_recurrent_kernel(const RecParams p) {
   constexpr int R = K / RG;
   constexpr int THREADS = VC / CPT * RG;
   constexpr int CL = 32 / RG;               // column groups per warp

@@ -10,8 +10,8 @@
 // exact in bf16 (448 2^119 is its largest, 2^-129 its smallest).  A row of zeros has e = 0; an infinity saturates to 448 2^e;
 // NaN stays NaN.  A bf16 cache takes the rows as they are.
 //
-// Both kernels are bound by memory: 8 values per lane (16-byte loads of bf16),
-// H / 8 lanes per row with the row maximum by shuffles.
+// Bound by memory: 8 values per lane (16-byte loads of bf16), H / 8 lanes per row
+// with the row maximum by shuffles.
 #include <cuda_fp8.h>
 #include <torch/extension.h>
 
@@ -21,6 +21,8 @@
 
 namespace hb {
 namespace {
+
+constexpr int U = 2;   // rows per thread
 
 struct RowStrides {   // in elements; the last dimension is contiguous
   long long b, s, n;
@@ -72,49 +74,74 @@ HB_DEVICE int row_exponent(float amax) {
   return min(max(e, -120), 119);
 }
 
+// A block covers NB heads (blockDim.x = NB * H / 8 lanes) of U * blockDim.y tokens
+// of one sequence (blockIdx.y); blockIdx.z is the side and the group of heads.
+// The places follow from the block's shape without a division: with flat row
+// numbers the divisions and their address arithmetic were most of the
+// instructions, and these bound the kernels.
+struct Where {
+  int side, b, n, l;   // l: lane within the row
+  unsigned i0;         // first token; then every blockDim.y-th
+};
+template <int H>
+HB_DEVICE Where where() {
+  constexpr int LPR = H / 8;
+  const int x = threadIdx.x, heads = blockDim.x / LPR;
+  return {(int)(blockIdx.z & 1), (int)blockIdx.y, (int)(blockIdx.z >> 1) * heads + x / LPR, x % LPR,
+          blockIdx.x * U * blockDim.y + threadIdx.y};
+}
+
 template <typename T, int H, bool QUANT>
-__global__ void __launch_bounds__(256) kv_write_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(1024) kv_write_kernel(const WriteParams p) {
   constexpr int LPR = H / 8;   // lanes per row
-  const WriteSide& sd = p.side[blockIdx.y];
-  const unsigned row = (blockIdx.x * 256u + threadIdx.x) / LPR;
-  const int l = threadIdx.x % LPR;
-  const unsigned n = row % p.N, bs = row / p.N, i = bs % p.S, b = bs / p.S;
-  bool on = b < p.B;
-  long long at = 0;
-  if (on) {
-    on = p.counts == nullptr || (int)i < p.counts[b];
-    at = (long long)p.starts[b] + i;
-    if (on) on = index_ok(at, p.C, p.status);
+  const Where w0 = where<H>();
+  const WriteSide& sd = p.side[w0.side];
+  const unsigned N = p.N, S = p.counts ? min((unsigned)max(p.counts[w0.b], 0), p.S) : p.S;
+  const int l = w0.l;
+  const bool head = (unsigned)w0.n < N;
+  const long long start = p.starts[w0.b];
+  const T* src = reinterpret_cast<const T*>(sd.x) + w0.b * sd.xs.b + w0.n * sd.xs.n + l * 8;
+  const long long out0 = w0.b * sd.cs.b + w0.n * sd.cs.n + l * 8, exp0 = w0.b * sd.es.b + w0.n * sd.es.n;
+  float f[U][8] = {};
+  long long at[U];
+  bool on[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {   // all loads before the first use
+    const unsigned i = w0.i0 + u * blockDim.y;
+    at[u] = start + i;
+    on[u] = head && i < S && index_ok(at[u], p.C, p.status);
+    if (on[u]) load8<T>(src + i * sd.xs.s, f[u]);
   }
-  float f[8] = {};
-  if (on) load8<T>(reinterpret_cast<const T*>(sd.x) + b * sd.xs.b + i * sd.xs.s + n * sd.xs.n + l * 8, f);
-  if constexpr (!QUANT) {
-    if (!on) return;
-    __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(sd.cache) + b * sd.cs.b + at * sd.cs.s + n * sd.cs.n + l * 8;
-    *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                                pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-  } else {
-    float amax = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float a = fabsf(f[j]);
-      if (a < INFINITY) amax = fmaxf(amax, a);   // false for NaN too
+  for (int u = 0; u < U; ++u) {
+    if constexpr (!QUANT) {
+      if (!on[u]) continue;
+      __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(sd.cache) + out0 + at[u] * sd.cs.s;
+      *reinterpret_cast<uint4*>(out) = make_uint4(pack_bf16x2(f[u][0], f[u][1]), pack_bf16x2(f[u][2], f[u][3]),
+                                                  pack_bf16x2(f[u][4], f[u][5]), pack_bf16x2(f[u][6], f[u][7]));
+    } else {
+      float amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float a = fabsf(f[u][j]);
+        if (a < INFINITY) amax = fmaxf(amax, a);   // false for NaN too
+      }
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (!on[u]) continue;
+      const int e = row_exponent(amax);
+      const float inv = pow2i(-e);
+      uint32_t w[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[u][4 * h] * inv, f[u][4 * h + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[u][4 * h + 2] * inv, f[u][4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+        w[h] = lo | (hi << 16);
+      }
+      uint8_t* out = reinterpret_cast<uint8_t*>(sd.cache) + out0 + at[u] * sd.cs.s;
+      *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+      if (l == 0) sd.exps[exp0 + at[u] * sd.es.s] = (int8_t)e;
     }
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (!on) return;
-    const int e = row_exponent(amax);
-    const float inv = pow2i(-e);
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h] * inv, f[4 * h + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h + 2] * inv, f[4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-      w[h] = lo | (hi << 16);
-    }
-    uint8_t* out = reinterpret_cast<uint8_t*>(sd.cache) + b * sd.cs.b + at * sd.cs.s + n * sd.cs.n + l * 8;
-    *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
-    if (l == 0) sd.exps[b * sd.es.b + at * sd.es.s + n * sd.es.n] = (int8_t)e;
   }
 }
 
@@ -141,42 +168,63 @@ HB_DEVICE uint2 unpack4(uint32_t w, float sc) {
 }
 
 template <int H, bool QUANT>
-__global__ void __launch_bounds__(256) kv_read_kernel(const ReadParams p) {
-  constexpr int LPR = H / 8;
-  const ReadSide& sd = p.side[blockIdx.y];
-  const unsigned row = (blockIdx.x * 256u + threadIdx.x) / LPR;
-  const int l = threadIdx.x % LPR;
-  const unsigned n = row % p.N, bs = row / p.N, i = bs % p.S, b = bs / p.S;
-  if (b >= p.B) return;
-  const long long at = (p.starts ? (long long)p.starts[b] : 0) + i;
-  uint4 o = make_uint4(0, 0, 0, 0);
-  if (index_ok(at, p.C, p.status)) {
-    const long long off = b * sd.cs.b + at * sd.cs.s + n * sd.cs.n + l * 8;
-    if constexpr (QUANT) {
-      const uint2 c = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(sd.cache) + off);
-      const float sc = pow2i(sd.exps[b * sd.es.b + at * sd.es.s + n * sd.es.n]);
-      const uint2 x = unpack4(c.x, sc), y = unpack4(c.y, sc);
-      o = make_uint4(x.x, x.y, y.x, y.y);
-    } else {
-      o = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(sd.cache) + off);
+__global__ void __launch_bounds__(1024) kv_read_kernel(const ReadParams p) {
+  const Where w0 = where<H>();
+  const ReadSide& sd = p.side[w0.side];
+  if ((unsigned)w0.n >= p.N) return;
+  const int l = w0.l;
+  const long long start = p.starts ? p.starts[w0.b] : 0;
+  const long long in0 = w0.b * sd.cs.b + w0.n * sd.cs.n + l * 8, exp0 = w0.b * sd.es.b + w0.n * sd.es.n;
+  __nv_bfloat16* out = sd.out + ((long long)w0.b * p.S * p.N + w0.n) * H + l * 8;
+  uint4 o[U] = {};
+  uint2 c[U] = {};
+  int e[U] = {};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {   // all loads before the first use
+    const unsigned i = w0.i0 + u * blockDim.y;
+    const long long at = start + i;
+    if (i < p.S && index_ok(at, p.C, p.status)) {
+      if constexpr (QUANT) {
+        c[u] = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(sd.cache) + in0 + at * sd.cs.s));
+        e[u] = __ldg(sd.exps + exp0 + at * sd.es.s);
+      } else {
+        o[u] = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(sd.cache) + in0 + at * sd.cs.s));
+      }
     }
   }
-  *reinterpret_cast<uint4*>(sd.out + ((long long)bs * p.N + n) * H + l * 8) = o;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const unsigned i = w0.i0 + u * blockDim.y;
+    if (i >= p.S) continue;
+    if constexpr (QUANT) {   // code 0 where there was no row
+      const float sc = pow2i(e[u]);
+      const uint2 x = unpack4(c[u].x, sc), y = unpack4(c[u].y, sc);
+      o[u] = make_uint4(x.x, x.y, y.x, y.y);
+    }
+    *reinterpret_cast<uint4*>(out + (long long)i * p.N * H) = o[u];
+  }
 }
 
 RowStrides strides_of(const torch::Tensor& t) { return {t.stride(0), t.stride(1), t.stride(2)}; }
 
 template <typename T, bool QUANT>
-void launch_write(const WriteParams& p, int H, dim3 grid) {
-  if (H == 32) kv_write_kernel<T, 32, QUANT><<<grid, 256, 0, cur_stream()>>>(p);
-  else if (H == 64) kv_write_kernel<T, 64, QUANT><<<grid, 256, 0, cur_stream()>>>(p);
-  else kv_write_kernel<T, 128, QUANT><<<grid, 256, 0, cur_stream()>>>(p);
+void launch_write(const WriteParams& p, int H, dim3 grid, dim3 block) {
+  if (H == 32) kv_write_kernel<T, 32, QUANT><<<grid, block, 0, cur_stream()>>>(p);
+  else if (H == 64) kv_write_kernel<T, 64, QUANT><<<grid, block, 0, cur_stream()>>>(p);
+  else kv_write_kernel<T, 128, QUANT><<<grid, block, 0, cur_stream()>>>(p);
 }
 
-dim3 rows_grid(int64_t rows, int64_t H) {
-  const int64_t per = 256 / (H / 8), blocks = (rows + per - 1) / per;
-  HB_CHECK(rows < (1ll << 31) && blocks < (1ll << 31), "kv_cache: too many rows for one call");
-  return dim3((unsigned)blocks, 2, 1);
+// Blocks of whole warps: up to 128 lanes of heads, about 256 threads.
+void shape_of(int64_t B, int64_t S, int64_t N, int64_t H, dim3& grid, dim3& block) {
+  const int64_t lpr = H / 8, heads = std::min(N, 128 / lpr), x = heads * lpr;
+  int64_t unit = 1;   // tokens that make whole warps
+  while (x * unit % 32) unit *= 2;
+  int64_t y = unit;
+  while (y * 2 * x <= 256 && y < S) y *= 2;
+  const int64_t groups = (N + heads - 1) / heads, blocks = (S + U * y - 1) / (U * y);
+  need(B <= 65535 && 2 * groups <= 65535 && blocks < (1ll << 31) && S < (1ll << 31), "kv_cache: too many rows for one call");
+  grid = dim3((unsigned)blocks, (unsigned)B, (unsigned)(2 * groups));
+  block = dim3((unsigned)x, (unsigned)y);
 }
 
 }  // namespace
@@ -209,13 +257,14 @@ void kv_cache_write(torch::Tensor k_cache, torch::Tensor v_cache, OptTensor k_ex
   p.counts = counts ? counts->data_ptr<int>() : nullptr;
   p.B = (unsigned)B, p.S = (unsigned)S, p.N = (unsigned)N, p.C = (int)k_cache.size(1);
   p.status = status_ptr();
-  const dim3 grid = rows_grid(B * S * N, H);
+  dim3 grid, block;
+  shape_of(B, S, N, H, grid, block);
   if (k.scalar_type() == at::kBFloat16) {
-    if (quant) launch_write<__nv_bfloat16, true>(p, (int)H, grid);
-    else launch_write<__nv_bfloat16, false>(p, (int)H, grid);
+    if (quant) launch_write<__nv_bfloat16, true>(p, (int)H, grid, block);
+    else launch_write<__nv_bfloat16, false>(p, (int)H, grid, block);
   } else {
-    if (quant) launch_write<float, true>(p, (int)H, grid);
-    else launch_write<float, false>(p, (int)H, grid);
+    if (quant) launch_write<float, true>(p, (int)H, grid, block);
+    else launch_write<float, false>(p, (int)H, grid, block);
   }
   HB_CUDA_CHECK(cudaGetLastError());
 }
@@ -241,16 +290,17 @@ std::tuple<torch::Tensor, torch::Tensor> kv_cache_read(torch::Tensor k_cache, to
   p.starts = starts ? starts->data_ptr<int>() : nullptr;
   p.B = (unsigned)B, p.S = (unsigned)S, p.N = (unsigned)N, p.C = (int)k_cache.size(1);
   p.status = status_ptr();
-  const dim3 grid = rows_grid(B * S * N, H);
+  dim3 grid, block;
+  shape_of(B, S, N, H, grid, block);
   const cudaStream_t st = cur_stream();
   if (quant) {
-    if (H == 32) kv_read_kernel<32, true><<<grid, 256, 0, st>>>(p);
-    else if (H == 64) kv_read_kernel<64, true><<<grid, 256, 0, st>>>(p);
-    else kv_read_kernel<128, true><<<grid, 256, 0, st>>>(p);
+    if (H == 32) kv_read_kernel<32, true><<<grid, block, 0, st>>>(p);
+    else if (H == 64) kv_read_kernel<64, true><<<grid, block, 0, st>>>(p);
+    else kv_read_kernel<128, true><<<grid, block, 0, st>>>(p);
   } else {
-    if (H == 32) kv_read_kernel<32, false><<<grid, 256, 0, st>>>(p);
-    else if (H == 64) kv_read_kernel<64, false><<<grid, 256, 0, st>>>(p);
-    else kv_read_kernel<128, false><<<grid, 256, 0, st>>>(p);
+    if (H == 32) kv_read_kernel<32, false><<<grid, block, 0, st>>>(p);
+    else if (H == 64) kv_read_kernel<64, false><<<grid, block, 0, st>>>(p);
+    else kv_read_kernel<128, false><<<grid, block, 0, st>>>(p);
   }
   HB_CUDA_CHECK(cudaGetLastError());
   return {k_out, v_out};
