@@ -10,13 +10,21 @@ KV / recurrent-state cache).
 
 Greedy decoding with the cache produces the same tokens as the reference's
 full recomputation (tests/test_train_cpu.py).
+
+:class:`BatchCache` and :func:`generate_batch` decode many sequences at once on
+the decoding operators (:mod:`hanuman_b200.ops`): a prompt that all of them share
+is run once and read by all; keys and values may be held in 8 bits; several
+drafted tokens a sequence are verified in one step.
 """
 from __future__ import annotations
 
 import numpy as np
 import torch
+import torch.nn.functional as F
 
+from . import ops
 from .models.transformer import Transformer
+from .ops import reference as ref
 
 
 class KVCache:
@@ -84,3 +92,279 @@ def generate_cached(model: Transformer, tokenizer, prompt: str, max_tokens: int 
             break
         logits = step(model, torch.tensor([[nxt]], device=dev), cache)
     return tokenizer.decode(generated), generated
+
+
+# ---------------------------------------------------------------------- batches
+class _AttentionRows:
+    """One attention layer of a :class:`BatchCache`."""
+
+    def __init__(self, owner, own: ops.KVCache, prefix):
+        self.owner, self.own, self.prefix = owner, own, prefix
+
+    def attend(self, q, k, v, window):
+        c = self.owner
+        ops.kv_cache_write(self.own, k, v, c.lengths, c.counts)
+        if c.fresh and c.counts is None and not self.own.quantised:
+            return ops.attention(q, k, v, window)          # a whole prompt at once
+        return ops.decode_attention(q, self.own, c.after, c.counts, self.prefix, window)
+
+
+class _KdaState:
+    """One KDA layer of a :class:`BatchCache`: the recurrent state and the
+    projected rows that the causal conv still sees.  ``advance`` runs new tokens;
+    the state moves on when the cache commits how many of them stay."""
+
+    def __init__(self, owner, state=None, hist=None):
+        self.owner, self.state, self.hist = owner, state, hist
+        self.pending = None
+
+    def advance(self, mod, h, dtype):
+        B, S, D = h.shape
+        H, K = mod.n_heads, mod.head_dim
+        taps = mod.q_conv.weight.shape[-1]
+        if self.hist is None:
+            self.hist = torch.zeros(1, taps - 1, 3 * H * K, dtype=torch.bfloat16 if h.is_cuda else dtype, device=h.device)
+        hist = self.hist.expand(B, -1, -1)
+        if h.is_cuda:
+            from .ops.kda import kda_out_cuda, kda_rows_cuda
+            q, k, v, g, beta, gl, rows = kda_rows_cuda(mod, h, hist)
+        else:
+            xf = h.reshape(B * S, D).float()
+            new = torch.cat([(xf @ w.float()).to(dtype) for w in (mod.wq, mod.wk, mod.wv)], dim=1).view(B, S, 3 * H * K)
+            rows = torch.cat([hist.to(dtype), new], dim=1)
+            conv = torch.cat([c.weight for c in (mod.q_conv, mod.k_conv, mod.v_conv)], dim=0)
+            x = F.silu(ref.short_conv(rows, conv)[:, taps - 1:].float())
+            q, k, v = (t.reshape(B, S, H, K) for t in x.split(H * K, dim=-1))
+            q, k = ref.l2_norm(q, 1e-6), ref.l2_norm(k, 1e-6)
+            f = ((xf @ mod.f_proj0.float()) @ mod.f_proj1.float()).view(B, S, H, K)
+            g = ref.kda_gate(f, mod.a_log, mod.dt_bias, mod.gate)
+            beta = torch.sigmoid(xf @ mod.wb.float()).view(B, S, H)
+        inputs = (q, k, v, g, beta, K ** -0.5)
+        o, state = ops.kda_recurrent(*inputs, state=self.state, counts=self.owner.counts)
+        self.pending = (inputs, state, rows, taps - 1)
+        if h.is_cuda:
+            return kda_out_cuda(mod, o, gl)
+        o = o * torch.rsqrt((o * o).mean(-1, keepdim=True) + 1e-5) * mod.o_norm
+        gate = torch.sigmoid((xf @ mod.g_proj0.float()) @ mod.g_proj1.float() + mod.g_proj1_bias).view(B, S, H, K)
+        return ((o * gate).reshape(B * S, H * K) @ mod.wo.float()).view(B, S, D)
+
+    def commit(self, kept):
+        inputs, state, rows, back = self.pending
+        if kept is None:
+            self.state = state
+            kept = self.owner.counts
+        else:   # fewer tokens stay than were run: run those alone
+            _, self.state = ops.kda_recurrent(*inputs, state=self.state, counts=kept)
+        if kept is None:
+            self.hist = rows[:, -back:].contiguous()
+        else:   # the last rows of the tokens that stay
+            at = kept.long()[:, None] + torch.arange(back, device=rows.device)
+            self.hist = torch.gather(rows, 1, at[..., None].expand(-1, -1, rows.shape[2]))
+        self.pending = None
+
+
+class BatchCache:
+    """Decoding state of a batch: per attention layer rows of keys and values
+    (``kv_dtype``: the model's type, or ``torch.float8_e4m3fn``), per KDA layer
+    the recurrent state.  ``lengths [B]`` counts each sequence's own tokens;
+    ``fork`` starts a batch behind this cache's one sequence without copying it."""
+
+    def __init__(self, model: Transformer, batch: int, capacity: int, kv_dtype=None, prefix: "BatchCache" = None):
+        dev, cfg = model.wte.device, model.cfg
+        self.batch, self.capacity = batch, capacity
+        self.prefix_len = 0 if prefix is None else prefix.host_length
+        self.kv_dtype = kv_dtype or (torch.bfloat16 if dev.type == "cuda" else model.dtype)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.max_pos = max(cfg.seq_len, cfg.infer_seq_len) - 1
+        self.counts, self.after = None, None
+        self.host_length = 0         # of the longest sequence, as far as the host knows
+        self.layers = {}
+        for i, blk in enumerate(model.blocks):
+            if blk.attention_type == "kda":
+                src = None if prefix is None else prefix.layers[i]
+                self.layers[i] = _KdaState(self, *(() if src is None else (src.state, src.hist)))
+            else:
+                own = ops.new_kv_cache(batch, capacity, cfg.n_kv_heads, cfg.head_dim, dev, self.kv_dtype)
+                shared = None if prefix is None else prefix.layers[i].own.rows(prefix.host_length)
+                self.layers[i] = _AttentionRows(self, own, shared)
+
+    @property
+    def fresh(self) -> bool:
+        """No token, own or shared, came before this step."""
+        return self.prefix_len == 0 and self.host_length == 0
+
+    def kv(self, layer: int):
+        return self.layers[layer]
+
+    def kda_state(self, layer: int):
+        return self.layers[layer]
+
+    def fork(self, model: Transformer, batch: int, capacity: int) -> "BatchCache":
+        """A batch whose sequences all continue this cache's one sequence."""
+        if self.batch != 1 or self.prefix_len or self.host_length == 0:
+            raise ValueError("fork: a cache of one sequence with tokens and no prefix of its own")
+        return BatchCache(model, batch, capacity, self.kv_dtype, prefix=self)
+
+    def run(self, model: Transformer, tokens: torch.Tensor, counts=None) -> torch.Tensor:
+        """Hidden states ``[B, S, D]`` of new tokens ``[B, S]``, of which a
+        sequence has ``counts[b]`` (all S without it).  :meth:`commit` follows."""
+        B, S = tokens.shape
+        if self.host_length + S > self.capacity:
+            raise ValueError(f"{self.host_length} + {S} tokens do not fit a capacity of {self.capacity}")
+        self.counts = None if counts is None else counts.to(torch.int32)
+        self.after = self.lengths + (S if counts is None else self.counts)
+        pos = self.prefix_len + self.lengths[:, None] + torch.arange(S, device=tokens.device)
+        self.new = S
+        return model(tokens, positions=pos.clamp(max=self.max_pos).long(), cache=self)[0]
+
+    def commit(self, kept=None):
+        """Keep the first ``kept[b]`` of the tokens just run (all without it)."""
+        for layer in self.layers.values():
+            if isinstance(layer, _KdaState):
+                layer.commit(kept)
+        self.lengths = self.after if kept is None else self.lengths + kept.to(torch.int32)
+        self.host_length += self.new
+        self.counts = self.after = None
+
+    def at_most(self, length: int):
+        """Tell the cache what the host has read: no sequence is longer."""
+        self.host_length = min(self.host_length, length)
+
+    def snapshot(self):
+        return self.lengths, self.host_length, {i: (x.state, x.hist) for i, x in self.layers.items() if isinstance(x, _KdaState)}
+
+    def restore(self, snap):
+        self.lengths, self.host_length, states = snap
+        for i, (state, hist) in states.items():
+            self.layers[i].state, self.layers[i].hist = state, hist
+
+
+def _last_logits(model, h, counts):
+    at = counts.long().clamp(min=1) - 1
+    return model.logits(h[torch.arange(h.shape[0], device=h.device), at])
+
+
+class _Sampler:
+    """Next tokens, with or without drafted ones, from a seeded generator."""
+
+    def __init__(self, batch, temperature, seed, device):
+        self.gen = torch.Generator(device=device).manual_seed(seed)
+        self.temperature = torch.full((batch,), float(max(temperature, 0.0)), device=device)
+        self.device = device
+
+    def verify(self, logits, drafted, draft_logits=None, lens=None):
+        B, K1, V = logits.shape
+        uniform = torch.rand(B, K1 - 1, generator=self.gen, device=self.device)
+        noise = torch.rand(B, V, generator=self.gen, device=self.device)
+        noise = (-torch.log1p(-noise)).clamp(min=1e-30)
+        return ops.verify_draft(logits, drafted, uniform, noise, draft_logits, lens, self.temperature)
+
+    def draw(self, logits):
+        none = torch.zeros(logits.shape[0], 0, dtype=torch.int64, device=self.device)
+        return self.verify(logits[:, None], none)[0][:, 0]
+
+
+def lookup_draft(ids, n: int):
+    """Up to n tokens that followed the latest earlier occurrence of the last two."""
+    for i in range(len(ids) - 3, -1, -1):
+        if ids[i:i + 2] == ids[-2:]:
+            return ids[i + 2:i + 2 + n]
+    return []
+
+
+@torch.no_grad()
+def generate_batch(model: Transformer, tokenizer, prompts, max_tokens: int = 100, temperature: float = 1.0,
+                   seed: int = 0, shared_prompt: str = "", kv_dtype=None, n_draft: int = 0,
+                   draft_model: Transformer = None):
+    """Decode ``prompts`` (each behind ``shared_prompt``, which runs once) together.
+
+    ``n_draft`` tokens a sequence are drafted and verified per step: by
+    ``draft_model``, or without one by looking up what followed the last two
+    tokens before.  Greedy output (``temperature`` 0) does not depend on the
+    drafts; sampled output keeps the target model's distribution.  Returns a list
+    of ``(text, ids)``, ids with the prompt's."""
+    dev = model.wte.device
+    B = len(prompts)
+    shared = tokenizer.encode(shared_prompt) if shared_prompt else []
+    rests = [tokenizer.encode(p) or ([] if shared else [0]) for p in prompts]
+    if shared and not all(rests):   # every sequence feeds a token of its own
+        shared, rests = shared[:-1], [shared[-1:] + r for r in rests]
+    longest = max(len(r) for r in rests)
+    capacity = longest + max_tokens + n_draft + 1
+
+    def prefill(m):
+        if shared:
+            one = BatchCache(m, 1, len(shared), kv_dtype)
+            one.run(m, torch.tensor([shared], device=dev))
+            one.commit()
+            cache = one.fork(m, B, capacity)
+        else:
+            cache = BatchCache(m, B, capacity, kv_dtype)
+        counts = torch.tensor([len(r) for r in rests], dtype=torch.int32, device=dev)
+        tokens = torch.tensor([r + [0] * (longest - len(r)) for r in rests], device=dev)
+        h = cache.run(m, tokens, counts)
+        cache.commit()
+        return cache, _last_logits(m, h, counts)
+
+    cache, logits = prefill(model)
+    draft_cache = prefill(draft_model)[0] if draft_model is not None and n_draft else None
+    sampler = _Sampler(B, temperature, seed, dev)
+    eos = getattr(tokenizer, "eos_id", None)
+    out = [list(shared) + r for r in rests]
+    made = [0] * B
+    live = [True] * B
+
+    def take(b, ids):
+        for t in ids:
+            if not live[b]:
+                return
+            out[b].append(t)
+            made[b] += 1
+            live[b] = made[b] < max_tokens and t != eos
+
+    cur = sampler.draw(logits)
+    for b, t in enumerate(cur.tolist()):
+        live[b] = max_tokens > 0
+        take(b, [t])
+    while any(live):
+        on = torch.tensor([int(x) for x in live], dtype=torch.int32, device=dev)
+        drafted, draft_logits, lens = None, None, on * 0
+        if n_draft and draft_cache is not None:
+            snap = draft_cache.snapshot()
+            tok, got, rows = cur, [], []
+            for _ in range(n_draft):
+                h = draft_cache.run(draft_model, tok[:, None], on)
+                draft_cache.commit()
+                rows.append(draft_model.logits(h[:, 0]))
+                tok = sampler.draw(rows[-1])
+                got.append(tok)
+            draft_cache.restore(snap)
+            drafted, draft_logits, lens = torch.stack(got, 1), torch.stack(rows, 1), on * n_draft
+        elif n_draft:
+            found = [lookup_draft(o, n_draft) if x else [] for o, x in zip(out, live)]
+            drafted = torch.tensor([f + [0] * (n_draft - len(f)) for f in found], dtype=torch.int64, device=dev).view(B, -1)
+            lens = torch.tensor([len(f) for f in found], dtype=torch.int32, device=dev)
+        if drafted is None:
+            drafted = torch.zeros(B, 0, dtype=torch.int64, device=dev)
+        fed = torch.cat([cur[:, None], drafted], dim=1)
+        h = cache.run(model, fed, on + lens)
+        tokens, accepted, _ = sampler.verify(model.logits(h), drafted, draft_logits, lens)
+        kept = (accepted.to(torch.int32) + 1) * on
+        if n_draft:
+            cache.commit(kept)
+        else:
+            cache.commit()
+        if draft_cache is not None:
+            draft_cache.run(draft_model, fed, kept)
+            draft_cache.commit()
+        rows = tokens.tolist()
+        n = accepted.tolist()
+        cur = tokens.gather(1, accepted[:, None])[:, 0].clamp(min=0)
+        for b in range(B):
+            if live[b]:
+                take(b, rows[b][:n[b] + 1])
+        longest_now = max(len(o) for o in out) - len(shared)
+        cache.at_most(longest_now)
+        if draft_cache is not None:
+            draft_cache.at_most(longest_now)
+    return [(tokenizer.decode(o), o) for o in out]

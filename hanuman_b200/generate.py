@@ -55,10 +55,8 @@ def generate_from_model(model: Transformer, config: Config, tokenizer, prompt: s
     return tokenizer.decode(generated), generated
 
 
-def load_for_generate(config: Config, prompt: str, max_tokens: int = 100,
-                      temperature: float = 1.0, top_k: int = 0, seed: int = 0,
-                      device: str = None, cached: bool = False):
-    """Latest checkpoint of ``config`` -> text (generate.py:20-68)."""
+def load_model(config: Config, device: str = None):
+    """The model of ``config``'s latest checkpoint, on its device."""
     path = latest_checkpoint(config)
     if path is None:
         raise FileNotFoundError(f"No checkpoint under {config.checkpoint_dir}/{config.name}. Train first.")
@@ -75,8 +73,29 @@ def load_for_generate(config: Config, prompt: str, max_tokens: int = 100,
     if dev != "cpu":
         from .engine import Engine
         Engine(model, config, torch.device(dev))   # attaches compute-dtype working copies
+    return model
+
+
+def load_for_generate(config: Config, prompt: str, max_tokens: int = 100,
+                      temperature: float = 1.0, top_k: int = 0, seed: int = 0,
+                      device: str = None, cached: bool = False):
+    """Latest checkpoint of ``config`` -> text (generate.py:20-68)."""
+    model = load_model(config, device)
     if cached:
         from .decode import generate_cached
         return generate_cached(model, get_tokenizer(config), prompt, max_tokens, temperature, top_k, seed)
     return generate_from_model(model, config, get_tokenizer(config), prompt, max_tokens,
                                temperature, top_k, seed)
+
+
+def load_for_generate_batch(config: Config, prompts, max_tokens: int = 100, temperature: float = 1.0, seed: int = 0,
+                            shared_prompt: str = "", kv: str = "model", n_draft: int = 0, draft_config: Config = None,
+                            device: str = None):
+    """Latest checkpoint of ``config`` -> one text per prompt, decoded as one batch
+    (:func:`hanuman_b200.decode.generate_batch`); ``kv`` "fp8" holds keys and
+    values in 8 bits; ``draft_config``'s latest checkpoint drafts tokens."""
+    from .decode import generate_batch
+    model = load_model(config, device)
+    draft = load_model(draft_config, device) if draft_config is not None else None
+    return generate_batch(model, get_tokenizer(config), prompts, max_tokens, temperature, seed, shared_prompt,
+                          torch.float8_e4m3fn if kv == "fp8" else None, n_draft, draft)

@@ -55,6 +55,19 @@ def cmd_generate(args):
     config = get_config(args.config)
     if args.yarn_factor is not None:
         config.yarn_factor = args.yarn_factor
+    if args.prompt_file:
+        from .generate import load_for_generate_batch
+        if args.top_k:
+            raise SystemExit("--prompt_file samples with the temperature alone (no --top_k)")
+        with open(args.prompt_file) as f:
+            prompts = [line.rstrip("\n") for line in f if line.strip()]
+        results = load_for_generate_batch(
+            config, prompts, args.max_tokens, args.temperature, args.seed, args.shared_prompt, args.kv, args.n_draft,
+            get_config(args.draft_config) if args.draft_config else None)
+        for i, (text, _) in enumerate(results):
+            print(f"=== Generated {i} ===")
+            print(text)
+        return
     text, ids = load_for_generate(config, args.prompt, args.max_tokens, args.temperature,
                                   args.top_k, args.seed, cached=args.cache)
     print("=== Generated ===")
@@ -122,6 +135,13 @@ def build_parser():
     g.add_argument("--yarn_factor", type=float, default=None)
     g.add_argument("--cache", action="store_true",
                    help="incremental decoding with KV / KDA-state caches (same tokens, no recompute)")
+    g.add_argument("--prompt_file", default=None,
+                   help="decode every line of this file as one batch (KV / KDA-state caches)")
+    g.add_argument("--shared_prompt", default="", help="text before every prompt of the batch, run once")
+    g.add_argument("--kv", default="model", choices=["model", "fp8"], help="type of the batch's cached keys and values")
+    g.add_argument("--n_draft", type=int, default=0,
+                   help="tokens drafted and verified per step (by lookup, or by --draft_config's checkpoint)")
+    g.add_argument("--draft_config", default=None, choices=list(PRESETS))
     g.set_defaults(func=cmd_generate)
     c = sub.add_parser("count", help="Print param counts")
     c.add_argument("--config", default="full_g4", choices=list(PRESETS))

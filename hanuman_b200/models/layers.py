@@ -74,9 +74,12 @@ class Attention(nn.Module):
         v = ops.linear(x2, self.wv, compute_dtype=dtype).view(B, S, self.n_kv, H)
         q, k = ops.apply_rope(q, k, cos.to(dtype), sin.to(dtype), positions)
         q_offset = 0
-        if cache is not None:
-            k, v, q_offset = cache.update(k, v)
-        o = ops.attention(q, k, v, self.window, q_offset)
+        if hasattr(cache, "attend"):   # a batch's cache writes the rows and attends over them itself
+            o = cache.attend(q, k, v, self.window)
+        else:
+            if cache is not None:
+                k, v, q_offset = cache.update(k, v)
+            o = ops.attention(q, k, v, self.window, q_offset)
         o = o.reshape(B * S, self.n_q * H)
         return ops.linear(o, self.wo, out_dtype=torch.float32, compute_dtype=dtype).view(B, S, D)
 
@@ -155,6 +158,8 @@ class KDA(nn.Module):
         if h.is_cuda and state is None:
             from ..ops.kda import kda_layer_cuda
             return kda_layer_cuda(self, h, dtype)
+        if hasattr(state, "advance"):   # a batch's recurrent state
+            return state.advance(self, h, dtype)
         x = h.reshape(B * S, D)
         xf = x.float()
         # fp32 projections rounded to the compute dtype before the conv

@@ -252,6 +252,57 @@ class KdaOutGateFn(torch.autograd.Function):
         return do, dgl, dw.to(ctx.dtypes[0]), dgb.to(ctx.dtypes[1])
 
 
+def kda_rows_cuda(mod, h, hist):
+    """What one decoding call of a KDA layer needs on the GPU: the recurrence's
+    rows for ``h [B, S, D]`` after the ``taps - 1`` projected rows ``hist [B,
+    taps - 1, 3 H K]`` that the causal conv still sees.
+
+    The front-end kernel convolves every sequence from a zero history, so it runs
+    over the history rows and the new ones together, and the history's results
+    are dropped.  Returns ``(q, k, v, g, beta, gl, rows)``; ``rows [B, taps - 1 +
+    S, 3 H K]`` are the projected rows with the history in front."""
+    B, S, D = h.shape
+    H, K = mod.n_heads, mod.head_dim
+    HK, T, dev = H * K, B * S, h.device
+    xb = _bf16(h.reshape(T, D))
+    P = hist.shape[1]
+    big = torch.empty(T, 3 * HK + 2 * K, dtype=torch.bfloat16, device=dev)
+    off = 0
+    for w in (mod.wq, mod.wk, mod.wv, mod.f_proj0, mod.g_proj0):
+        _gemm_or_narrow(xb, _work(w), big[:, off:off + w.shape[1]], False, False, False)
+        off += w.shape[1]
+    f32 = dict(dtype=torch.float32, device=dev)
+    braw, f, gl = torch.empty(T, H, **f32), torch.empty(T, HK, **f32), torch.empty(T, HK, **f32)
+    _gemm_or_narrow(xb, _work(mod.wb), braw, False, False, False)
+    _gemm_or_narrow(big[:, 3 * HK:3 * HK + K], _work(mod.f_proj1), f, False, False, False)
+    _gemm_or_narrow(big[:, 3 * HK + K:], _work(mod.g_proj1), gl, False, False, False)
+    rows = torch.cat([hist, big[:, :3 * HK].view(B, S, 3 * HK)], dim=1)
+
+    def behind(x):   # [B, S, C] with P rows of zeros in front, flat
+        return torch.cat([x.new_zeros(B, P, x.shape[-1]), x.view(B, S, -1)], dim=1).view(B * (P + S), -1)
+
+    q = torch.empty(B * (P + S), H, K, **f32)
+    k, v, g = torch.empty_like(q), torch.empty_like(q), torch.empty_like(q)
+    beta = torch.empty(B * (P + S), H, **f32)
+    conv = [c.weight.float().contiguous() for c in (mod.q_conv, mod.k_conv, mod.v_conv)]
+    ext().kda_prep_fwd(rows.view(B * (P + S), 3 * HK), *conv, behind(f), mod.a_log.float().contiguous(),
+                       mod.dt_bias.float().contiguous(), behind(braw), 0 if mod.gate == "kimi" else 1, P + S,
+                       q, k, v, g, beta)
+    new = [t.view(B, P + S, *t.shape[1:])[:, P:] for t in (q, k, v, g, beta)]
+    return (*new, gl, rows)
+
+
+def kda_out_cuda(mod, o, gl):
+    """Output norm, gate and projection of the recurrence's ``o [B, S, H, K]``."""
+    B, S, H, K = o.shape
+    if K in (32, 64, 128):
+        y = KdaOutGateFn.apply(o.view(B * S, H, K), gl, mod.o_norm, mod.g_proj1_bias)
+    else:
+        on = o * torch.rsqrt((o * o).mean(-1, keepdim=True) + 1e-5) * mod.o_norm
+        y = (on * torch.sigmoid(gl + mod.g_proj1_bias).view(B, S, H, K)).reshape(B * S, H * K).to(torch.bfloat16)
+    return linear_fused(y, [mod.wo], torch.float32).view(B, S, -1)
+
+
 def kda_layer_cuda(mod, h, dtype):
     B, S, D = h.shape
     T = B * S
