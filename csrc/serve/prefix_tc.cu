@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(Tc<H, NS>::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + NS);
 
   launch_dependents();
-  const int warp = threadIdx.x / 32;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int R = p.B * p.S * p.G, SG = p.S * p.G;
   const long long total = (long long)p.N * p.tc_rt * p.tc_tiles;
   const long long t_begin = (long long)blockIdx.x * p.tc_per;
@@ -212,6 +212,9 @@ __global__ void __launch_bounds__(Tc<H, NS>::THREADS, 1)
       if (ok) ok = mbar_wait(smem_u32(bar), parity, p.status, kErrTimeoutEpilogue, p.budget_ns);
       ok = __all_sync(0xffffffffu, ok);
     };
+    if constexpr (NS == 2) {
+      if (st == 1) asm volatile("bar.arrive 1, 256;" ::: "memory");   // stream 0 begins
+    }
     int it = 0;
     while (it < n_it) {   // pieces
       const long long tile = t_begin + it;
@@ -221,15 +224,26 @@ __global__ void __launch_bounds__(Tc<H, NS>::THREADS, 1)
       const int rr = rt * (NS * 128) + st * 128 + r;
       const bool real = rr < R;
       int lo = 0;
-      {   // this thread's row of Q into the swizzled K-major tile
+      {
+        // Rows of Q into the swizzled K-major tile: H / 8 lanes read a row, so a
+        // warp reads whole lines (a row per lane took 4500 cycles for 64 columns)
         const int b = real ? rr / SG : 0, ri = real ? rr % SG : 0, i = ri / p.G;
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + b * p.qb + i * p.qs + (long long)(n * p.G + ri % p.G) * p.qh);
-        const uint32_t row = sQ + st * F::Q_BYTES + r * 128;
+        const long long mine = b * p.qb + i * p.qs + (long long)(n * p.G + ri % p.G) * p.qh;   // row 0 where there is none
+        constexpr int LPR = H / 8, RPI = 32 / LPR;
+        uint4 x[32 / RPI];
 #pragma unroll
-        for (int c = 0; c < H / 8; ++c) {
-          const uint4 x = real ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (c >> 3) * 128 * 128 + (((c & 7) ^ (r & 7)) << 4)),
-                       "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
+        for (int k = 0; k < 32 / RPI; ++k) {   // all loads before the first store
+          const long long off = __shfl_sync(0xffffffffu, mine, k * RPI + lane / LPR);
+          x[k] = __ldg(reinterpret_cast<const uint4*>(p.q + off) + lane % LPR);
+        }
+        const int first = rr - lane, c = lane % LPR;
+#pragma unroll
+        for (int k = 0; k < 32 / RPI; ++k) {
+          const int row = (r & ~31) + k * RPI + lane / LPR;
+          if (first + k * RPI + lane / LPR >= R) x[k] = make_uint4(0, 0, 0, 0);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                           sQ + st * F::Q_BYTES + row * 128 + (c >> 3) * 128 * 128 + (((c & 7) ^ (row & 7)) << 4)),
+                       "r"(x[k].x), "r"(x[k].y), "r"(x[k].z), "r"(x[k].w)
                        : "memory");
         }
         if (p.W > 0 && real) {
@@ -290,6 +304,10 @@ __global__ void __launch_bounds__(Tc<H, NS>::THREADS, 1)
             }
           }
         }
+        // The exponentials of the two streams take turns: each then has the
+        // special-function units alone while the other reads its next scores and
+        // finds their maximum (in step, both did: 3370 cycles a tile).
+        if constexpr (NS == 2) asm volatile("bar.sync %0, 256;" ::"r"(1 + st) : "memory");
         const float nm = m == -INFINITY ? 0.f : -m;
         const uint64_t sl2_2 = pack2(p.sl2, p.sl2), nm_2 = pack2(nm, nm);
         uint64_t ls[2] = {0, 0};
@@ -306,6 +324,9 @@ __global__ void __launch_bounds__(Tc<H, NS>::THREADS, 1)
           }
           tmem_st_x16(tP + 16 * c, w);
         }
+        if constexpr (NS == 2) {
+          if (st == 0 || it + 1 < n_it) asm volatile("bar.arrive %0, 256;" ::"r"(2 - st) : "memory");
+        }
         float l0, l1;
         unpack2(add2(ls[0], ls[1]), l0, l1);
         l += l0 + l1;
@@ -316,19 +337,32 @@ __global__ void __launch_bounds__(Tc<H, NS>::THREADS, 1)
       wait(&pv_done[st], (it - 1) & 1);
       tc_fence_after();
       const long long at = ((long long)blockIdx.x + u) * (NS * 128) + st * 128 + r;
+      // O by 32 columns through the warp's 4 KB of the stream's Q tile (its scores
+      // are done), so that a warp writes whole lines
+      const uint32_t box = sQ + st * F::Q_BYTES + (r >> 5) * 4096;
 #pragma unroll
       for (int c = 0; c < H / 32; ++c) {
         uint32_t v[32];
         tmem_ld_32x32b_x32(tO + 32 * c, v);
         tmem_ld_wait();
-        if (real && ok) {
-          float4* o = reinterpret_cast<float4*>(p.pre_o + at * H + 32 * c);
+        __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            o[e] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]), __uint_as_float(v[4 * e + 2]),
-                               __uint_as_float(v[4 * e + 3]));
+        for (int e = 0; e < 8; ++e)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 128 + ((e ^ (lane & 7)) << 4)), "r"(v[4 * e]),
+                       "r"(v[4 * e + 1]), "r"(v[4 * e + 2]), "r"(v[4 * e + 3])
+                       : "memory");
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int row = 4 * k + lane / 8, e = lane % 8;
+          uint4 y;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                       : "r"(box + row * 128 + ((e ^ (row & 7)) << 4)) : "memory");
+          if (rr - lane + row < R && ok)
+            *reinterpret_cast<uint4*>(p.pre_o + (at - lane + row) * H + 32 * c + 4 * e) = y;
         }
       }
+      __syncwarp();
       if (real) *reinterpret_cast<float2*>(p.pre_ml + at * 2) = make_float2(m, l);
       tc_fence_before();
     }
