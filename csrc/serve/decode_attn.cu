@@ -515,8 +515,12 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 && MT == 1 && H <= 64 ? 2 : 1
             r0 = pack_f16x2(x0 * r[0] * wv[i][0], x1 * r[0] * wv[i][1]);
             r1 = pack_f16x2(x2 * r[1] * wv[i][0], x3 * r[1] * wv[i][1]);
           } else {
+            // P as two bf16 terms: one alone would add as much error as the output's
+            // own rounding; the second product is a tenth of a tile's instructions
             r0 = pack_bf16x2(x0, x1);
             r1 = pack_bf16x2(x2, x3);
+            s[mt][i][2] = __uint_as_float(pack_bf16x2(x0 - __uint_as_float(r0 << 16), x1 - __uint_as_float(r0 & 0xffff0000u)));
+            s[mt][i][3] = __uint_as_float(pack_bf16x2(x2 - __uint_as_float(r1 << 16), x3 - __uint_as_float(r1 & 0xffff0000u)));
           }
           s[mt][i][0] = __uint_as_float(r0), s[mt][i][1] = __uint_as_float(r1);
         }
@@ -531,6 +535,11 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 && MT == 1 && H <= 64 ? 2 : 1
           a[mt] = make_uint4(__float_as_uint(s[mt][2 * k][0]), __float_as_uint(s[mt][2 * k][1]),
                              __float_as_uint(s[mt][2 * k + 1][0]), __float_as_uint(s[mt][2 * k + 1][1]));
         if constexpr (!Q8) {
+          uint4 a2[MT];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            a2[mt] = make_uint4(__float_as_uint(s[mt][2 * k][2]), __float_as_uint(s[mt][2 * k][3]),
+                                __float_as_uint(s[mt][2 * k + 1][2]), __float_as_uint(s[mt][2 * k + 1][3]));
 #pragma unroll
           for (int jn = 0; jn < JN; jn += 2) {
             uint32_t r[4];
@@ -539,6 +548,8 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 && MT == 1 && H <= 64 ? 2 : 1
             for (int mt = 0; mt < MT; ++mt) {
               mma_bf16(O[mt][jn], a[mt], r[0], r[1]);
               mma_bf16(O[mt][jn + 1], a[mt], r[2], r[3]);
+              mma_bf16(O[mt][jn], a2[mt], r[0], r[1]);
+              mma_bf16(O[mt][jn + 1], a2[mt], r[2], r[3]);
             }
           }
         } else {
