@@ -26,6 +26,11 @@
 // through shared memory at the end of a piece.  Products on mma.sync: at S * G
 // rows the tensor work is small against the bytes of the keys.
 //
+// Bound by a warp's chain through a tile (a thousand cycles with 4 of 16 rows in
+// use), then by memory.  Measured on a B200, head dim 64, 16 query and 4 KV heads:
+// 64 sequences of 1 to 1024 keys 13.2 us in either type (8-bit: 17 MB, bf16: 34 MB),
+// 256 of them 38 us (8-bit, 67 MB); one sequence of 4096 keys 9.4 us, of 32768 11.6.
+//
 // A quantised cache holds e4m3 codes and a power-of-two exponent per row.  The
 // codes convert to f16 exactly.  q (bf16) enters as f16 scaled per row by a power
 // of two to [2^14, 2^15): exact but for values 2^-25 below the row's largest.
@@ -162,7 +167,7 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 && MT == 1 && H <= 64 ? 2 : 1
       for (int w = 0; w < NW; ++w) total += wsum[w];
     }
     if (report && tid == 0) p.tile_start[p.B] = total;
-    const int per = max(NW, (total + p.n_suf - 1) / p.n_suf);
+    const int per = max(1, (total + p.n_suf - 1) / p.n_suf);
     tile0 = min(c * per, total), tile1 = min(tile0 + per, total);
     if (tile0 >= tile1) return;
     // second walk: every warp finds the sequence by itself
@@ -729,7 +734,7 @@ __global__ void __launch_bounds__(128) decode_combine_kernel(const AttnParams p)
     n = h / p.G, g = h % p.G;
     const int len = len_of(p, b, false);
     live = i < count_of(p, b, len, false);
-    const int total = p.tile_start[p.B], per = max(WARPS, (total + p.n_suf - 1) / p.n_suf);
+    const int total = p.tile_start[p.B], per = max(1, (total + p.n_suf - 1) / p.n_suf);
     const int t0 = p.tile_start[b], t1 = p.tile_start[b + 1];
     c_lo = t0 / per;
     own_n = t1 > t0 ? (t1 - 1) / per - c_lo + 1 : 0;
@@ -890,19 +895,30 @@ torch::Tensor decode_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v
   const int SG = p.S * p.G, R = p.B * SG;
   const int sms = num_sms();
   p.budget_ns = wait_budget_ns();
-  // Many rows that share the prefix: tcgen05 (128-row tiles); few: mma.sync.
-  const bool tc = p.P && H >= 64 && R > 64;
+  // Many rows that share the prefix: tcgen05 (128-row tiles, keys read once); few:
+  // mma.sync in the same launch as the own keys (each tile of 32 rows reads the
+  // keys again).  us on mma.sync and on tcgen05, prefix 4096 / 32768: bf16, 16 rows
+  // 11.6 and 12.0 / 19.2 and 24.0, 32 rows 14.5 and 12.4 / 26.5 and 24.4; 8-bit
+  // (whose tcgen05 way first writes the values out), 32 rows 15.6 and 15.2 / 27.2
+  // and 34.6, 64 rows 16.6 and 17.2 / 32.9 and 34.7, 128 rows 23.4 and 18.3 / 48.2 and 35.7.
+  const bool tc = p.P && H >= 64 && R > (q8 ? 32 : 16);
   const int mt = SG > 16 || (p.P && !tc && R > 16) ? 2 : 1;
   p.own_rt = (SG + 16 * mt - 1) / (16 * mt);
-  // One CTA per (sequence, KV head) when those fill half the SMs and no sequence
-  // is long: it joins the prefix pieces itself (one launch less).  Not where
-  // the prefix runs on mma.sync, in the same launch as the own keys.
-  const bool whole = (!p.P || tc) && (long long)p.B * p.N * p.own_rt >= sms / 2 && p.C <= 2048;
+  // One CTA per (sequence, KV head) that joins the prefix pieces itself (one launch
+  // less), unless sequences may be long: up to 512 keys, or 2048 where the CTAs
+  // fill half the SMs.  Against shares and a join in a second launch, us: 19
+  // sequences of up to 512 keys 6.8 and 13.2, 2048 14.0 and 14.4, 4096 24.6 and
+  // 18.4; 64 of up to 2048 22.2 and 27.7.  Not where the prefix runs on mma.sync,
+  // in the same launch as the own keys.
+  const bool whole = (!p.P || tc) && (p.C <= 512 || ((long long)p.B * p.N * p.own_rt >= sms / 2 && p.C <= 2048));
   // eight warps a CTA where four would take more than two tiles each
   const bool wide = p.C > 256;
-  // own keys: about two CTAs per SM, at least 8 tiles of the full capacity each
+  // Shares of the own keys: about two CTAs per SM, 8 tiles each when the sequences
+  // are full, but as many as there are sequences (a share of several runs them
+  // one after the other, some 4 us each).
   const long long cap_tiles = (long long)p.B * ((p.C + KB - 1) / KB);
-  p.n_suf = (int)std::max<long long>(1, std::min<long long>(2ll * sms / ((long long)p.N * p.own_rt), cap_tiles / 8));
+  p.n_suf = (int)std::max<long long>(
+      1, std::min<long long>(2ll * sms / ((long long)p.N * p.own_rt), std::max<long long>(p.B, cap_tiles / 8)));
   long long pre_rows = 0;
   if (p.P) p.pre_lo = p.W > 0 ? std::max(0, p.P - p.W + 1) : 0;
   if (tc) {

@@ -19,6 +19,9 @@
 // at the start.  One launch, no workspace.
 //
 // Bound by memory: 2 K + 1 rows of V logits and one row of noise per sequence.
+// Measured on a B200: 128 sequences, 7 drafts, 32768 fp32 logits (268 MB) 67 us, of
+// which reading the rows takes 46 (5.5 TB/s) and the joins and the race the rest;
+// one sequence with 4 drafts 9.4 us, nearly all of it the chain of phases.
 #include <torch/extension.h>
 
 #include "../common/host.h"
